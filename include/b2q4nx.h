@@ -64,7 +64,8 @@ int b2_set_launch_options(int pdl);
 /* Read and clear the device error word (0 = none; the first error wins): 1-4 a
  * bounded wait gave up (1 full-wait, 2 empty-wait, 3 drain; 4 unused), 5 an
  * attention call met a sequence position outside its cache or planned length, 6 a
- * tensor-parallel exchange waited too long for another rank (b2_tp_*).
+ * tensor-parallel exchange waited too long for another rank (b2_tp_*), 7 a page pool had
+ * no free page left (b2_kv4_reorder).
  * Synchronises `stream`.  Returns B2_OK or B2_ERR_CUDA. */
 int b2_read_device_error(int* code, void* stream);
 
@@ -387,6 +388,110 @@ int b2_q4_swiglu_gemm_rmsnorm(const uint8_t* gate, const uint8_t* up, int n_tile
  *   gu fp32 [batch][ldgu], 16-byte aligned, ldgu % 4 == 0, ldgu >= 2K. */
 int b2_q4_gemm_swiglu_in(const uint8_t* tiles, int n_tile_rows, int k_tiles, const float* gu, int batch, int ldgu,
                           float* y, int ldy, int flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The 4-bit paged KV cache.  No reference counterpart: the reference keeps K and V in
+ * bf16 (designs/granite_gemv/granite_attention.h:80-213).
+ *
+ * A page holds `page` tokens (a multiple of 16, at most 4096) of every kv head: pool
+ * uint8 [n_pages][n_kv_heads][page / 16][head_dim / 64][1152], 16-byte aligned.  A
+ * 1152-byte cell is 16 tokens x 64 dims of K and V: codes of 4 bits and, per token and
+ * 64 dims, a bf16 pair (d, m); a value is code * d + m, 4.5 bits each in all.  The byte
+ * order inside a cell is given in llmnputest_b200/csrc/kv4_cell.cuh.
+ *   table    int32 [batch][max_pages]: the page of the pool that holds tokens
+ *            j*page .. of the sequence, -1 where there is none
+ *   summary  bf16 [n_pages][n_kv_heads][2][head_dim]: least and largest key per dim of
+ *            each page (after rotation), or null
+ *   pos      int32 [batch], as in b2_gqa_decode; -1 marks a sequence without tokens (a
+ *            padded batch row)
+ *   head_dim 64, 128 or 256; n_q_heads / n_kv_heads <= 8.
+ * A position outside the table, or an entry outside the pool where a page is needed,
+ * records device error 5; nothing is read or written for it.  Device error 7: the pool
+ * had no free page left (b2_kv4_reorder). */
+#define B2_KV4_NO_ROPE 1  /* keys or queries are not rotated */
+#define B2_KV4_OUT_F32 2  /* b2_kv4_decode: fp32 output */
+#define B2_KV4_ROWS_F32 4 /* append, gather: rows are fp32 (else bf16) */
+
+/* Quantise new rows into the pool.  k, v [rows][ld], kv head h at h*head_dim.  Sequence b
+ * has rows cu[b] .. cu[b+1]-1 (cu int32 [batch+1], ascending, 0 .. rows; null: row b
+ * alone), which become its tokens pos[b], pos[b]+1, ...: k is rotated to its position
+ * (half-split RoPE as b2_gqa_decode), and per token, kv head and 64 dims
+ *   m = bf16(min x), d = max(bf16((max x - m) / 15), 2^-40),
+ *   code = clamp(floor((x - m) / d + 1/2), 0, 15),
+ * evaluated in fp64.  64 values of which one is not finite read back as NaN.  A page whose
+ * first token is among the rows gets a new summary, else the keys join the old one.  Rows
+ * outside cu, and the tokens beside the new ones, are left as they are.  Two sequences of a
+ * call may not share a page that either writes. */
+int b2_kv4_append(const void* k, const void* v, int64_t ld_k, int64_t ld_v, int rows, uint8_t* pool,
+                  const int32_t* table, const int32_t* pos, const int32_t* cu, uint16_t* summary, int batch,
+                  int n_kv_heads, int head_dim, int page, int max_pages, int n_pages, float theta, int flags,
+                  void* stream);
+
+/* Read rows back: code * d + m of tokens pos[b], pos[b]+1, ... into rows cu[b] ..
+ * cu[b+1]-1 of k and v (16-byte aligned rows).  Rows that no token goes to keep what they
+ * hold. */
+int b2_kv4_gather(void* k, void* v, int64_t ld_k, int64_t ld_v, int rows, const uint8_t* pool, const int32_t* table,
+                  const int32_t* pos, const int32_t* cu, int batch, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int flags, void* stream);
+
+/* Decode attention of one query per sequence over tokens 0..pos[b] of the cache (the new
+ * token's k and v already appended): q fp32 [batch][ld_q], head j at j*head_dim, rotated
+ * to pos[b]; out bf16 (fp32 with B2_KV4_OUT_F32) [batch][ldo]; zeros where pos[b] is -1.
+ * With sel (int32 [batch][n_kv_heads][n_sel] page indices in ascending order, as
+ * b2_kv4_select lists them) only the tokens of those pages are attended, per kv head; an
+ * entry that is negative, behind pos[b] or not above the entry before it counts for
+ * nothing.  Without sel, n_sel is 0.  max_len >= max(pos) + 1 sizes the split.
+ * q enters the products as fp16 (scaled by a power of two per head), the weights as fp16
+ * against fp32 sums.  workspace: 16-byte aligned. */
+int b2_kv4_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page, int n_sel,
+                                 int max_len, size_t* bytes);
+int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32_t* table, const int32_t* pos,
+                  const int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int max_len, float theta, float scale, void* out, int64_t ldo,
+                  void* workspace, size_t workspace_bytes, int flags, void* stream);
+
+/* The pages a query attends to: per (sequence, kv head) the n_sel pages of 0..pos[b] whose
+ * bound max_j sum_d max(q_jd lo_d, q_jd hi_d) over the kv head's q heads is largest (q
+ * rotated; lo, hi the page's summary; in fp64).  The page of pos[b] is always listed, and
+ * of two equal bounds the lower page goes first.  sel [batch][n_kv_heads][n_sel] ascending,
+ * filled up with -1.  At most 16384 pages (max_len / page). */
+int b2_kv4_select_workspace_size(int batch, int n_kv_heads, int page, int max_len, size_t* bytes);
+int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const int32_t* table, const int32_t* pos,
+                  int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int max_len, float theta, void* workspace, size_t workspace_bytes,
+                  int flags, void* stream);
+
+/* Pages across the layers of a cache: pool [layers][n_pages][page_bytes], and summary
+ * [layers][n_pages][summary_bytes] or null (bytes of a page, multiples of 16).  refs int32
+ * [n_pages]: how many table entries hold a page; 0 marks a free page.
+ *
+ * b2_kv4_copy_pages: page src[i] to dst[i], i < n <= 65535, in every layer.  Entries that
+ * are negative or equal are skipped.  The destinations are distinct, and none is a source. */
+int b2_kv4_copy_pages(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers,
+                      int n_pages, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* b2_kv4_reorder: the rows of a page table anew.  Row b goes on with the tokens of row
+ * parent[b] (-1: with none), lens[parent[b]] of them, and is given pages for reserve[b]
+ * more (reserve null: none).  Full pages are shared (refs counts them); the first row of a
+ * parent keeps its last, partly filled page and those behind it, every further one gets a
+ * copy of the former; pages that no row holds any longer are free.  Pages are given out
+ * from the lowest free one up, in order of the rows.  If they run out, the entries that
+ * are left stay -1, a row that misses the copy of its last page is cut to its full pages,
+ * and device error 7 is recorded.  info int32 [4]: free pages left, pages copied, pages
+ * missing, 0.  The outputs are not the inputs' buffers. */
+int b2_kv4_reorder_workspace_size(int batch, int max_pages, int n_pages, size_t* bytes);
+int b2_kv4_reorder(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers, int n_pages,
+                   const int32_t* table, const int32_t* lens, const int32_t* refs, const int32_t* parent,
+                   const int32_t* reserve, int batch, int max_pages, int page, int32_t* table_out, int32_t* lens_out,
+                   int32_t* refs_out, int32_t* info, void* workspace, size_t workspace_bytes, void* stream);
+
+/* b2_kv4_compact: live pages to the lowest numbers: of n live pages those at n and above
+ * move, the k-th of them to the k-th free page below n; table entries and refs follow.
+ * info int32 [4]: live pages, pages moved, 0, 0.  The outputs are not the inputs' buffers. */
+int b2_kv4_compact_workspace_size(int n_pages, size_t* bytes);
+int b2_kv4_compact(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers, int n_pages,
+                   const int32_t* table, const int32_t* refs, int batch, int max_pages, int32_t* table_out,
+                   int32_t* refs_out, int32_t* info, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1378,3 +1378,5 @@ int b2_q8_dequant_matrix(const uint8_t* tiles, int n_tile_rows, int k_tiles, flo
 }
 
 }  // extern "C"
+
+#include "kv4_entry.cuh"

@@ -1,0 +1,474 @@
+// C entry points of the 4-bit paged KV cache (b2_kv4_*): argument checks, launch plans.
+// Part of the library's one translation unit; uses its device_info, fail and cuda_fail.
+#pragma once
+
+#include <cmath>
+
+#include "kv4_append.cuh"
+#include "kv4_decode.cuh"
+#include "kv4_pages.cuh"
+#include "kv4_select.cuh"
+
+namespace {
+
+constexpr int kKv4MaxSelectPages = 16384;  // the keys of one (sequence, kv head) in 128 KB of shared memory
+
+struct Kv4Shape {
+  int batch, hkv, head_dim, page, max_pages, n_pages;
+};
+
+int kv4_check(const Kv4Shape& s) {
+  if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256)
+    return fail(B2_ERR_ARG, "head_dim %d: 64, 128 and 256 are built", s.head_dim);
+  if (s.batch < 1 || s.batch > 65535) return fail(B2_ERR_ARG, "batch %d outside 1..65535", s.batch);
+  if (s.hkv < 1 || s.hkv > 65535) return fail(B2_ERR_ARG, "n_kv_heads %d outside 1..65535", s.hkv);
+  if (s.page < 16 || s.page % 16 || s.page > 4096)
+    return fail(B2_ERR_ARG, "page %d: a multiple of 16, at most 4096, is needed", s.page);
+  if (s.max_pages < 1 || s.n_pages < 1) return fail(B2_ERR_ARG, "empty page table or pool");
+  if (static_cast<long long>(s.max_pages) * s.page > (1LL << 30))
+    return fail(B2_ERR_ARG, "a page table over more than 2^30 tokens");
+  return B2_OK;
+}
+
+int kv4_heads(int hq, int hkv) {
+  if (hq < 1 || hq % hkv) return fail(B2_ERR_ARG, "bad head counts hq=%d hkv=%d", hq, hkv);
+  if (hq / hkv > b2::kKv4MaxGroup) return fail(B2_ERR_ARG, "GQA group %d > 8 is not supported", hq / hkv);
+  return B2_OK;
+}
+
+// the angles' table of (theta, head_dim), made once per thread for calls with the same two
+const b2::Kv4Rope& kv4_rope(float theta, int head_dim, int flags) {
+  static thread_local b2::Kv4Rope off = {}, on = {};
+  static thread_local float on_theta = 0.f;
+  static thread_local int on_dim = 0;
+  if (flags & B2_KV4_NO_ROPE) return off;
+  if (on_theta != theta || on_dim != head_dim) {
+    for (int i = 0; i < head_dim / 2; ++i)
+      on.turn[i] = std::pow(static_cast<double>(theta), -2.0 * i / head_dim) / 6.283185307179586476925287;
+    on.on = 1;
+    on_theta = theta;
+    on_dim = head_dim;
+  }
+  return on;
+}
+
+struct Kv4Launch {
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = {};
+  Kv4Launch(dim3 grid, int threads, void* stream, size_t smem = 0) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_for(kPdlOther) ? 1 : 0;
+  }
+};
+
+// head_dim as a template argument
+template <typename F>
+auto kv4_by_dim(int head_dim, F f) {
+  return head_dim == 64    ? f(std::integral_constant<int, 64>())
+         : head_dim == 128 ? f(std::integral_constant<int, 128>())
+                           : f(std::integral_constant<int, 256>());
+}
+
+struct Kv4DecodePlan {
+  int tiles, n_splits, split_tiles;
+  size_t ws_bytes;
+};
+
+// Tiles of 16 tokens split over CTAs until there are about four per SM, no split below 8 tiles.
+Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int tokens, int sms) {
+  Kv4DecodePlan pl;
+  pl.tiles = (tokens + 15) / 16;
+  const long long pairs = static_cast<long long>(batch) * hkv;
+  const long long most = std::max(1, pl.tiles / 8);
+  const long long s = std::max(1LL, std::min(most, (4LL * sms + pairs - 1) / pairs));
+  pl.split_tiles = static_cast<int>((pl.tiles + s - 1) / s);
+  pl.n_splits = (pl.tiles + pl.split_tiles - 1) / pl.split_tiles;
+  pl.ws_bytes = pl.n_splits > 1 ? static_cast<size_t>(batch) * hq * pl.n_splits * (head_dim + 2) * sizeof(float) : 0;
+  return pl;
+}
+
+// tokens that a call's splits cover: those of the selected pages, or max_len
+int kv4_decode_tokens(int n_sel, int page, int max_len) {
+  return n_sel > 0 ? n_sel * page : max_len;
+}
+
+}  // namespace
+
+extern "C" {
+
+static int kv4_rows_call(bool append, const void* k, const void* v, int64_t ld_k, int64_t ld_v, int rows, void* pool,
+                         const int32_t* table, const int32_t* pos, const int32_t* cu, uint16_t* summary,
+                         const Kv4Shape& s, float theta, int flags, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  st = kv4_check(s);
+  if (st != B2_OK) return st;
+  if (!pool || !table || !pos) return fail(B2_ERR_ARG, "null pointer argument");
+  if (flags & ~(append ? B2_KV4_NO_ROPE | B2_KV4_ROWS_F32 : B2_KV4_ROWS_F32)) return fail(B2_ERR_ARG, "unknown flags 0x%x", flags);
+  if (rows < 0) return fail(B2_ERR_ARG, "negative row count");
+  if (!cu && rows != s.batch) return fail(B2_ERR_ARG, "%d rows for %d sequences: row offsets are needed", rows, s.batch);
+  if (append && !(flags & B2_KV4_NO_ROPE) && !(theta > 0.f)) return fail(B2_ERR_ARG, "theta must be > 0");
+  if (rows == 0) return B2_OK;
+  if (!k || !v) return fail(B2_ERR_ARG, "null pointer argument");
+  const int64_t width = static_cast<int64_t>(s.hkv) * s.head_dim;
+  if (rows > 1 && (ld_k < width || ld_v < width)) return fail(B2_ERR_ARG, "row stride below n_kv_heads * head_dim");
+  if (!aligned(pool, 16)) return fail(B2_ERR_ALIGN, "the pool must be 16-byte aligned");
+  const int f32 = (flags & B2_KV4_ROWS_F32) ? 1 : 0;
+  if (!append) {  // rows stored 16 bytes at a time
+    const int64_t per = f32 ? 4 : 8;
+    if (!aligned(k, 16) || !aligned(v, 16) || (rows > 1 && (ld_k % per || ld_v % per)))
+      return fail(B2_ERR_ALIGN, "gathered rows must be 16-byte aligned");
+  }
+  b2::Kv4RowsParams p = {};
+  p.k = k;
+  p.v = v;
+  p.ld_k = ld_k;
+  p.ld_v = ld_v;
+  p.pool = static_cast<uint8_t*>(pool);
+  p.table = table;
+  p.pos = pos;
+  p.cu = cu;
+  p.summary = reinterpret_cast<__nv_bfloat16*>(summary);
+  p.rows = rows;
+  p.batch = s.batch;
+  p.hkv = s.hkv;
+  p.page = s.page;
+  p.max_pages = s.max_pages;
+  p.n_pages = s.n_pages;
+  p.is_f32 = f32;
+  // a sequence of n rows touches at most n / page + 2 pages
+  const int jobs = cu ? rows / s.page + 2 * s.batch : s.batch;
+  Kv4Launch l(dim3(jobs, s.hkv, 1), b2::kKv4AppendThreads, stream);
+  const b2::Kv4Rope& rope = kv4_rope(theta, s.head_dim, append ? flags : B2_KV4_NO_ROPE);
+  const cudaError_t e = kv4_by_dim(s.head_dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (append) return cudaLaunchKernelEx(&l.cfg, b2::kv4_append_kernel<D>, p, rope);
+    return f32 ? cudaLaunchKernelEx(&l.cfg, b2::kv4_gather_kernel<D, float>, p)
+               : cudaLaunchKernelEx(&l.cfg, b2::kv4_gather_kernel<D, __nv_bfloat16>, p);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, append ? "kv4 append launch" : "kv4 gather launch");
+  return B2_OK;
+}
+
+int b2_kv4_append(const void* k, const void* v, int64_t ld_k, int64_t ld_v, int rows, uint8_t* pool,
+                  const int32_t* table, const int32_t* pos, const int32_t* cu, uint16_t* summary, int batch,
+                  int n_kv_heads, int head_dim, int page, int max_pages, int n_pages, float theta, int flags,
+                  void* stream) {
+  return kv4_rows_call(true, k, v, ld_k, ld_v, rows, pool, table, pos, cu, summary,
+                       {batch, n_kv_heads, head_dim, page, max_pages, n_pages}, theta, flags, stream);
+}
+
+int b2_kv4_gather(void* k, void* v, int64_t ld_k, int64_t ld_v, int rows, const uint8_t* pool, const int32_t* table,
+                  const int32_t* pos, const int32_t* cu, int batch, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int flags, void* stream) {
+  return kv4_rows_call(false, k, v, ld_k, ld_v, rows, const_cast<uint8_t*>(pool), table, pos, cu, nullptr,
+                       {batch, n_kv_heads, head_dim, page, max_pages, n_pages}, 0.f, flags, stream);
+}
+
+static int kv4_decode_check(const Kv4Shape& s, int hq, int n_sel, int max_len) {
+  int st = kv4_check(s);
+  if (st != B2_OK) return st;
+  st = kv4_heads(hq, s.hkv);
+  if (st != B2_OK) return st;
+  if (n_sel < 0 || n_sel > s.max_pages) return fail(B2_ERR_ARG, "n_sel %d outside 0..max_pages %d", n_sel, s.max_pages);
+  if (max_len < 1 || max_len > static_cast<long long>(s.max_pages) * s.page)
+    return fail(B2_ERR_ARG, "max_len %d outside 1..max_pages * page", max_len);
+  return B2_OK;
+}
+
+int b2_kv4_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page, int n_sel,
+                                 int max_len, size_t* bytes) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
+  if (max_len < 1 || page < 1 || n_sel < 0) return fail(B2_ERR_ARG, "bad lengths");
+  st = kv4_decode_check({batch, n_kv_heads, head_dim, page, std::max(n_sel, (max_len - 1) / page + 1), 1}, n_q_heads,
+                        n_sel, max_len);
+  if (st != B2_OK) return st;
+  *bytes = kv4_decode_plan(batch, n_q_heads, n_kv_heads, head_dim, kv4_decode_tokens(n_sel, page, max_len), di.sms).ws_bytes;
+  return B2_OK;
+}
+
+int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32_t* table, const int32_t* pos,
+                  const int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int max_len, float theta, float scale, void* out, int64_t ldo,
+                  void* workspace, size_t workspace_bytes, int flags, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  if ((sel == nullptr) != (n_sel == 0)) return fail(B2_ERR_ARG, "sel and n_sel go together");
+  st = kv4_decode_check({batch, n_kv_heads, head_dim, page, max_pages, n_pages}, n_q_heads, n_sel, max_len);
+  if (st != B2_OK) return st;
+  if (!q || !pool || !table || !pos || !out) return fail(B2_ERR_ARG, "null pointer argument");
+  if (flags & ~(B2_KV4_NO_ROPE | B2_KV4_OUT_F32)) return fail(B2_ERR_ARG, "unknown flags 0x%x", flags);
+  if (!(flags & B2_KV4_NO_ROPE) && !(theta > 0.f)) return fail(B2_ERR_ARG, "theta must be > 0");
+  const int64_t width = static_cast<int64_t>(n_q_heads) * head_dim;
+  if (batch > 1 && (ld_q < width || ldo < width)) return fail(B2_ERR_ARG, "row stride below n_q_heads * head_dim");
+  if (!aligned(pool, 16)) return fail(B2_ERR_ALIGN, "the pool must be 16-byte aligned");
+  const Kv4DecodePlan pl =
+      kv4_decode_plan(batch, n_q_heads, n_kv_heads, head_dim, kv4_decode_tokens(n_sel, page, max_len), di.sms);
+  if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)))
+    return fail(B2_ERR_WORKSPACE, "kv4 decode needs %zu bytes of 16-byte aligned workspace", pl.ws_bytes);
+  b2::Kv4DecodeParams p = {};
+  p.q = q;
+  p.ld_q = ld_q;
+  p.pool = pool;
+  p.table = table;
+  p.pos = pos;
+  p.sel = sel;
+  p.out = out;
+  p.part = static_cast<float*>(workspace);
+  p.ldo = ldo;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.batch = batch;
+  p.hq = n_q_heads;
+  p.hkv = n_kv_heads;
+  p.page = page;
+  p.max_pages = max_pages;
+  p.n_pages = n_pages;
+  p.n_sel = n_sel;
+  p.n_splits = pl.n_splits;
+  p.split_tiles = pl.split_tiles;
+  p.max_tiles = pl.tiles;
+  p.out_f32 = (flags & B2_KV4_OUT_F32) ? 1 : 0;
+  const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
+  Kv4Launch l(dim3(pl.n_splits, n_kv_heads, batch), b2::kKv4DecodeWarps * 32, stream);
+  cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
+    return cudaLaunchKernelEx(&l.cfg, b2::kv4_decode_kernel<decltype(d)::value>, p, rope);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 decode launch");
+  if (pl.n_splits > 1) {
+    Kv4Launch c(dim3(n_q_heads, batch, 1), head_dim, stream);
+    e = kv4_by_dim(head_dim, [&](auto d) {
+      return cudaLaunchKernelEx(&c.cfg, b2::kv4_combine_kernel<decltype(d)::value>, p);
+    });
+    if (e != cudaSuccess) return cuda_fail(e, "kv4 combine launch");
+  }
+  return B2_OK;
+}
+
+static int kv4_select_check(int page, int n_sel, int max_len, int* key_pages) {
+  if (page < 1 || max_len < 1) return fail(B2_ERR_ARG, "bad lengths");
+  *key_pages = (max_len - 1) / page + 1;
+  if (n_sel < 1) return fail(B2_ERR_ARG, "n_sel must be >= 1");
+  if (*key_pages > kKv4MaxSelectPages)
+    return fail(B2_ERR_ARG, "selection among %d pages: at most %d", *key_pages, kKv4MaxSelectPages);
+  return B2_OK;
+}
+
+int b2_kv4_select_workspace_size(int batch, int n_kv_heads, int page, int max_len, size_t* bytes) {
+  if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
+  int pages;
+  const int st = kv4_select_check(page, 1, max_len, &pages);
+  if (st != B2_OK) return st;
+  if (batch < 1 || n_kv_heads < 1) return fail(B2_ERR_ARG, "empty batch");
+  *bytes = static_cast<size_t>(batch) * n_kv_heads * pages * sizeof(unsigned long long);
+  return B2_OK;
+}
+
+int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const int32_t* table, const int32_t* pos,
+                  int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
+                  int max_pages, int n_pages, int max_len, float theta, void* workspace, size_t workspace_bytes,
+                  int flags, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  st = kv4_decode_check({batch, n_kv_heads, head_dim, page, max_pages, n_pages}, n_q_heads, 0, max_len);
+  if (st != B2_OK) return st;
+  int pages;
+  st = kv4_select_check(page, n_sel, max_len, &pages);
+  if (st != B2_OK) return st;
+  if (!q || !summary || !table || !pos || !sel) return fail(B2_ERR_ARG, "null pointer argument");
+  if (flags & ~B2_KV4_NO_ROPE) return fail(B2_ERR_ARG, "unknown flags 0x%x", flags);
+  if (!(flags & B2_KV4_NO_ROPE) && !(theta > 0.f)) return fail(B2_ERR_ARG, "theta must be > 0");
+  if (batch > 1 && ld_q < static_cast<int64_t>(n_q_heads) * head_dim)
+    return fail(B2_ERR_ARG, "row stride below n_q_heads * head_dim");
+  const size_t need = static_cast<size_t>(batch) * n_kv_heads * pages * sizeof(unsigned long long);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(B2_ERR_WORKSPACE, "kv4 select needs %zu bytes of 16-byte aligned workspace", need);
+  b2::Kv4SelectParams p = {};
+  p.q = q;
+  p.ld_q = ld_q;
+  p.summary = reinterpret_cast<const __nv_bfloat16*>(summary);
+  p.table = table;
+  p.pos = pos;
+  p.sel = sel;
+  p.key = static_cast<unsigned long long*>(workspace);
+  p.batch = batch;
+  p.hq = n_q_heads;
+  p.hkv = n_kv_heads;
+  p.page = page;
+  p.max_pages = max_pages;
+  p.n_pages = n_pages;
+  p.n_sel = n_sel;
+  p.key_pages = pages;
+  const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
+  Kv4Launch l(dim3((pages + b2::kKv4ScorePages - 1) / b2::kKv4ScorePages, n_kv_heads, batch), b2::kKv4ScoreThreads,
+              stream);
+  cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
+    return cudaLaunchKernelEx(&l.cfg, b2::kv4_score_kernel<decltype(d)::value>, p, rope);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 select launch (bounds)");
+  const size_t smem = static_cast<size_t>(pages) * sizeof(unsigned long long);
+  if (smem > 40 * 1024) {
+    e = cudaFuncSetAttribute(b2::kv4_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kKv4MaxSelectPages * static_cast<int>(sizeof(unsigned long long)));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(kv4 pick)");
+  }
+  Kv4Launch c(dim3(n_kv_heads, batch, 1), b2::kKv4PickThreads, stream, smem);
+  e = cudaLaunchKernelEx(&c.cfg, b2::kv4_pick_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 select launch (choice)");
+  return B2_OK;
+}
+
+static int kv4_page_data(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers,
+                         int n_pages, b2::Kv4PageData* d) {
+  if (!pool) return fail(B2_ERR_ARG, "null pool");
+  if (layers < 1 || layers > 65535 || n_pages < 1) return fail(B2_ERR_ARG, "bad pool: %d layers of %d pages", layers, n_pages);
+  if (page_bytes < 16 || page_bytes % 16 || (summary && (summary_bytes < 16 || summary_bytes % 16)))
+    return fail(B2_ERR_ARG, "the bytes of a page must be a multiple of 16");
+  if (!aligned(pool, 16) || !aligned(summary, 16)) return fail(B2_ERR_ALIGN, "pool and summaries must be 16-byte aligned");
+  d->base[0] = pool;
+  d->bytes[0] = static_cast<unsigned long long>(page_bytes);
+  d->base[1] = summary;
+  d->bytes[1] = summary ? static_cast<unsigned long long>(summary_bytes) : 0;
+  d->layers = layers;
+  d->n_pages = n_pages;
+  return B2_OK;
+}
+
+// CTAs that share one page's bytes: each thread about four 16-byte pieces
+static int kv4_copy_parts(const b2::Kv4PageData& d) {
+  return static_cast<int>(std::min<unsigned long long>(64, (d.bytes[0] + d.bytes[1] + 16383) / 16384));
+}
+
+int b2_kv4_copy_pages(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers,
+                      int n_pages, const int32_t* src, const int32_t* dst, int n, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  b2::Kv4PageData d;
+  st = kv4_page_data(pool, page_bytes, summary, summary_bytes, layers, n_pages, &d);
+  if (st != B2_OK) return st;
+  if (n < 0 || n > 65535) return fail(B2_ERR_ARG, "%d copies: 0..65535", n);
+  if (n == 0) return B2_OK;
+  if (!src || !dst) return fail(B2_ERR_ARG, "null pointer argument");
+  Kv4Launch l(dim3(kv4_copy_parts(d), layers, n), b2::kKv4CopyThreads, stream);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, b2::kv4_copy_kernel, d, static_cast<const int*>(src), static_cast<const int*>(dst));
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 copy launch");
+  return B2_OK;
+}
+
+// need, copy, totals, then the free pages found
+static size_t kv4_reorder_ws(int batch, int max_pages, int n_pages) {
+  const size_t ids = std::min(static_cast<size_t>(batch) * max_pages, static_cast<size_t>(n_pages));
+  return (2 * static_cast<size_t>(batch) + 2 + ids) * sizeof(int);
+}
+
+int b2_kv4_reorder_workspace_size(int batch, int max_pages, int n_pages, size_t* bytes) {
+  if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
+  if (batch < 1 || max_pages < 1 || n_pages < 1) return fail(B2_ERR_ARG, "empty page table or pool");
+  *bytes = kv4_reorder_ws(batch, max_pages, n_pages);
+  return B2_OK;
+}
+
+int b2_kv4_reorder(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers, int n_pages,
+                   const int32_t* table, const int32_t* lens, const int32_t* refs, const int32_t* parent,
+                   const int32_t* reserve, int batch, int max_pages, int page, int32_t* table_out, int32_t* lens_out,
+                   int32_t* refs_out, int32_t* info, void* workspace, size_t workspace_bytes, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  b2::Kv4ReorderParams p = {};
+  st = kv4_page_data(pool, page_bytes, summary, summary_bytes, layers, n_pages, &p.data);
+  if (st != B2_OK) return st;
+  if (batch < 1 || batch > 65535 || max_pages < 1 || page < 1) return fail(B2_ERR_ARG, "bad page table shape");
+  if (!table || !lens || !refs || !parent || !table_out || !lens_out || !refs_out || !info)
+    return fail(B2_ERR_ARG, "null pointer argument");
+  if (table == table_out || lens == lens_out || refs == refs_out)
+    return fail(B2_ERR_ARG, "the new rows need buffers of their own");
+  const size_t need = kv4_reorder_ws(batch, max_pages, n_pages);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(B2_ERR_WORKSPACE, "kv4 reorder needs %zu bytes of 16-byte aligned workspace", need);
+  p.table = table;
+  p.lens = lens;
+  p.refs = refs;
+  p.parent = parent;
+  p.reserve = reserve;
+  p.table_out = table_out;
+  p.lens_out = lens_out;
+  p.refs_out = refs_out;
+  p.info = info;
+  p.need = static_cast<int*>(workspace);
+  p.copy = p.need + batch;
+  p.totals = p.copy + batch;
+  p.free_ids = p.totals + 2;
+  p.batch = batch;
+  p.max_pages = max_pages;
+  p.page = page;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(refs_out, refs, static_cast<size_t>(n_pages) * sizeof(int), cudaMemcpyDeviceToDevice, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(info, 0, 4 * sizeof(int), s);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder set-up");
+  Kv4Launch a(dim3(batch, 1, 1), b2::kKv4CopyThreads, stream);
+  e = cudaLaunchKernelEx(&a.cfg, b2::kv4_reorder_rows_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (rows)");
+  Kv4Launch f(dim3(1, 1, 1), b2::kKv4ScanThreads, stream);
+  e = cudaLaunchKernelEx(&f.cfg, b2::kv4_reorder_free_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (free pages)");
+  Kv4Launch c(dim3(kv4_copy_parts(p.data), batch, layers), b2::kKv4CopyThreads, stream);
+  e = cudaLaunchKernelEx(&c.cfg, b2::kv4_reorder_fill_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (copies)");
+  return B2_OK;
+}
+
+int b2_kv4_compact_workspace_size(int n_pages, size_t* bytes) {
+  if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
+  if (n_pages < 1) return fail(B2_ERR_ARG, "empty pool");
+  *bytes = 3 * static_cast<size_t>(n_pages) * sizeof(int);
+  return B2_OK;
+}
+
+int b2_kv4_compact(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t summary_bytes, int layers, int n_pages,
+                   const int32_t* table, const int32_t* refs, int batch, int max_pages, int32_t* table_out,
+                   int32_t* refs_out, int32_t* info, void* workspace, size_t workspace_bytes, void* stream) {
+  DevInfo di;
+  int st = device_info(&di);
+  if (st != B2_OK) return st;
+  b2::Kv4CompactParams p = {};
+  st = kv4_page_data(pool, page_bytes, summary, summary_bytes, layers, n_pages, &p.data);
+  if (st != B2_OK) return st;
+  if (batch < 1 || max_pages < 1) return fail(B2_ERR_ARG, "bad page table shape");
+  if (!table || !refs || !table_out || !refs_out || !info) return fail(B2_ERR_ARG, "null pointer argument");
+  if (table == table_out || refs == refs_out) return fail(B2_ERR_ARG, "the new rows need buffers of their own");
+  const size_t need = 3 * static_cast<size_t>(n_pages) * sizeof(int);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(B2_ERR_WORKSPACE, "kv4 compact needs %zu bytes of 16-byte aligned workspace", need);
+  p.table = table;
+  p.refs = refs;
+  p.table_out = table_out;
+  p.refs_out = refs_out;
+  p.info = info;
+  p.to = static_cast<int*>(workspace);
+  p.src = p.to + n_pages;
+  p.dst = p.src + n_pages;
+  p.batch = batch;
+  p.max_pages = max_pages;
+  Kv4Launch a(dim3(1, 1, 1), b2::kKv4ScanThreads, stream);
+  cudaError_t e = cudaLaunchKernelEx(&a.cfg, b2::kv4_compact_plan_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 compact launch (plan)");
+  Kv4Launch c(dim3(8 * di.sms, 1, 1), b2::kKv4CopyThreads, stream);
+  e = cudaLaunchKernelEx(&c.cfg, b2::kv4_compact_move_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 compact launch (moves)");
+  return B2_OK;
+}
+
+}  // extern "C"

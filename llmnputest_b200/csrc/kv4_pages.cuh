@@ -1,0 +1,286 @@
+// The pages of the 4-bit KV cache as rows of a page table hold them: forking, freeing,
+// reserving (reorder), compacting and copying.  Everything is decided on the device, from
+// the reference counts alone: a page is free when no row holds it (refs 0), and of the free
+// pages the lowest are given out first, in the order of the rows, so that the outcome does
+// not turn on the order in which CTAs run (the counts are whole numbers).
+#pragma once
+
+#include "kv4_cell.cuh"
+
+namespace b2 {
+
+// What a page is made of: `rows` arrays (layers) of the pool and of the summaries.
+struct Kv4PageData {
+  uint8_t* base[2];            // the pool, the summaries (or null)
+  unsigned long long bytes[2];  // of one page in one layer, multiples of 16
+  int layers, n_pages;
+};
+
+// One page of one layer from src to dst, by the whole CTA.
+__device__ __forceinline__ void kv4_copy_page(const Kv4PageData& d, int layer, int src, int dst, int part, int parts) {
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    if (!d.base[a]) continue;
+    const size_t n = d.bytes[a] / 16;
+    const uint4* from = reinterpret_cast<const uint4*>(d.base[a] + (static_cast<size_t>(layer) * d.n_pages + src) * d.bytes[a]);
+    uint4* to = reinterpret_cast<uint4*>(d.base[a] + (static_cast<size_t>(layer) * d.n_pages + dst) * d.bytes[a]);
+    for (size_t i = static_cast<size_t>(part) * blockDim.x + threadIdx.x; i < n; i += static_cast<size_t>(parts) * blockDim.x)
+      to[i] = from[i];
+  }
+}
+
+constexpr int kKv4CopyThreads = 256;
+constexpr int kDevNoPage = 7;  // the pool had no free page left
+
+// Copies of listed pages: grid (parts, layers, pairs).  Entries outside the pool are skipped.
+__global__ void __launch_bounds__(kKv4CopyThreads) kv4_copy_kernel(const Kv4PageData d, const int* src, const int* dst) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int s = src[blockIdx.z], t = dst[blockIdx.z];
+  if (s < 0 || t < 0 || s == t) return;
+  if (s >= d.n_pages || t >= d.n_pages) {
+    if (threadIdx.x == 0) record_error(kDevBadPosition);
+    return;
+  }
+  kv4_copy_page(d, blockIdx.y, s, t, blockIdx.x, gridDim.x);
+}
+
+// Sum of v over the threads below this one; total = over all (blockDim.x threads, 32 warps at most).
+__device__ __forceinline__ int kv4_block_before(int v, int* warps, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += x;
+  }
+  __syncthreads();  // the array's last use is over
+  if (lane == 31) warps[warp] = s;
+  __syncthreads();
+  int x = lane < nw ? warps[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  total = __shfl_sync(0xffffffffu, x, 31);
+  const int before = __shfl_sync(0xffffffffu, x, max(warp - 1, 0));
+  return s - v + (warp ? before : 0);
+}
+
+struct Kv4ReorderParams {
+  Kv4PageData data;
+  const int *table, *lens, *refs, *parent, *reserve;  // reserve may be null
+  int *table_out, *lens_out, *refs_out, *info;        // info[4]: free pages left, copied, missing, 0
+  int* need;  // [batch] pages each row lacks, then their sums below each row
+  int* copy;  // [batch] 0, or 1 + which of the row's missing pages is a copy of its parent's last one
+  int* free_ids;  // [total needed] at most batch * max_pages
+  int* totals;    // [2]: pages needed, pages found
+  int batch, max_pages, page;
+};
+
+// Row b's new entries, counts, and how many pages it lacks.  One CTA per row; refs_out holds
+// the old counts.
+__global__ void __launch_bounds__(kKv4CopyThreads) kv4_reorder_rows_kernel(const Kv4ReorderParams p) {
+  __shared__ int sh_first, sh_lack, sh_below;
+  const int b = blockIdx.x, tid = threadIdx.x, n_pages = p.data.n_pages;
+  pdl_wait();
+  pdl_launch_dependents();
+  int par = p.parent[b];
+  if (par < -1 || par >= p.batch) {
+    if (tid == 0) record_error(kDevBadPosition);
+    par = -1;
+  }
+  if (tid == 0) {
+    sh_first = 1;
+    sh_lack = sh_below = 0;
+  }
+  __syncthreads();
+  if (par >= 0)
+    for (int i = tid; i < b; i += kKv4CopyThreads)
+      if (p.parent[i] == par) sh_first = 0;
+  __syncthreads();
+  const bool first = sh_first != 0;
+  const int len = par >= 0 ? max(p.lens[par], 0) : 0;
+  const int full = len / p.page;
+  const long long tokens = static_cast<long long>(len) + (p.reserve ? max(p.reserve[b], 0) : 0);
+  const long long want = (tokens + p.page - 1) / p.page;
+  const int* mine = p.table + static_cast<size_t>(b) * p.max_pages;
+  const int* theirs = p.table + static_cast<size_t>(max(par, 0)) * p.max_pages;
+  int* out = p.table_out + static_cast<size_t>(b) * p.max_pages;
+  int lack = 0, below = 0;
+  for (int j = tid; j < p.max_pages; j += kKv4CopyThreads) {
+    const int old = mine[j];
+    if (old >= 0 && old < n_pages) atomicSub(&p.refs_out[old], 1);
+    int id = par >= 0 && (first || j < full) ? theirs[j] : -1;
+    if (id >= n_pages) id = -1;
+    if (id >= 0) atomicAdd(&p.refs_out[id], 1);
+    else id = -1;
+    out[j] = id;
+    lack += id < 0 && j < want;
+    below += id < 0 && j < full;
+  }
+  if (lack) atomicAdd(&sh_lack, lack);
+  if (below) atomicAdd(&sh_below, below);
+  __syncthreads();
+  if (tid == 0) {
+    p.need[b] = sh_lack;
+    const bool copies = par >= 0 && !first && len % p.page != 0 && full < p.max_pages && theirs[full] >= 0 &&
+                        theirs[full] < n_pages;
+    p.copy[b] = copies ? 1 + sh_below : 0;
+    p.lens_out[b] = len;
+    if (want > p.max_pages) {
+      record_error(kDevNoPage);
+      atomicAdd(&p.info[2], static_cast<int>(min(want - p.max_pages, 0x7FFFFFFFll)));
+    }
+  }
+}
+
+constexpr int kKv4ScanThreads = 1024;
+
+// One CTA: sums of the rows' needs, and the lowest free pages in order.
+__global__ void __launch_bounds__(kKv4ScanThreads) kv4_reorder_free_kernel(const Kv4ReorderParams p) {
+  __shared__ int warps[32];
+  const int tid = threadIdx.x, n_pages = p.data.n_pages;
+  pdl_wait();
+  pdl_launch_dependents();
+  int total = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += kKv4ScanThreads) {
+    const int b = b0 + tid, v = b < p.batch ? p.need[b] : 0;
+    int sum;
+    const int before = kv4_block_before(v, warps, sum);
+    if (b < p.batch) p.need[b] = total + before;
+    total += sum;
+  }
+  int found = 0;
+  for (int i0 = 0; i0 < n_pages; i0 += 4 * kKv4ScanThreads) {
+    const int i = i0 + 4 * tid;
+    int free4 = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < n_pages && p.refs_out[i + e] == 0) free4 |= 1 << e;
+    int sum, rank = found + kv4_block_before(__popc(free4), warps, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (free4 >> e & 1) {
+        if (rank < total) {
+          p.free_ids[rank] = i + e;
+          p.refs_out[i + e] = 1;
+        }
+        ++rank;
+      }
+    found += sum;
+  }
+  if (tid == 0) {
+    p.totals[0] = total;
+    p.totals[1] = min(found, total);
+    p.info[0] = found - min(found, total);
+    if (found < total) {
+      record_error(kDevNoPage);
+      atomicAdd(&p.info[2], total - found);
+    }
+  }
+}
+
+// Row blockIdx.y's missing pages filled in (CTAs of layer 0, part 0) and its parent's last
+// page copied: grid (parts, batch, layers).
+__global__ void __launch_bounds__(kKv4CopyThreads) kv4_reorder_fill_kernel(const Kv4ReorderParams p) {
+  __shared__ int warps[32];
+  const int b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int found = p.totals[1], rank0 = p.need[b];
+  const int par = p.parent[b];
+  const int copy_rank = rank0 + p.copy[b] - 1;
+  const bool copies = p.copy[b] != 0;
+  if (blockIdx.x == 0 && layer == 0) {
+    int* out = p.table_out + static_cast<size_t>(b) * p.max_pages;
+    const int len = p.lens_out[b];
+    const long long want = (static_cast<long long>(len) + (p.reserve ? max(p.reserve[b], 0) : 0) + p.page - 1) / p.page;
+    const int end = static_cast<int>(min(want, static_cast<long long>(p.max_pages)));
+    int rank = rank0;
+    for (int j0 = 0; j0 < end; j0 += kKv4CopyThreads) {
+      const int j = j0 + tid;
+      const int hole = j < end && out[j] < 0;
+      int sum;
+      const int at = rank + kv4_block_before(hole, warps, sum);
+      if (hole && at < found) out[j] = p.free_ids[at];
+      rank += sum;
+    }
+    __syncthreads();
+    if (tid == 0 && copies) {
+      if (copy_rank >= found) p.lens_out[b] = len / p.page * p.page;  // its last page could not be had
+      else atomicAdd(&p.info[1], 1);
+    }
+  }
+  if (!copies || copy_rank >= found) return;
+  const int src = p.table[static_cast<size_t>(par) * p.max_pages + p.lens[par] / p.page];
+  kv4_copy_page(p.data, layer, src, p.free_ids[copy_rank], blockIdx.x, gridDim.x);
+}
+
+struct Kv4CompactParams {
+  Kv4PageData data;
+  const int *table, *refs;
+  int *table_out, *refs_out, *info;  // info[4]: live pages, pages moved, 0, 0
+  int *to;         // [n_pages] where each live page goes
+  int *src, *dst;  // [n_pages] the moves
+  int batch, max_pages;
+};
+
+// One CTA: live pages counted, then the k-th free page below their number takes the k-th
+// live page at or above it.
+__global__ void __launch_bounds__(kKv4ScanThreads) kv4_compact_plan_kernel(const Kv4CompactParams p) {
+  __shared__ int warps[32];
+  const int tid = threadIdx.x, n = p.data.n_pages;
+  pdl_wait();
+  pdl_launch_dependents();
+  int mine = 0, live;
+  for (int i = tid; i < n; i += kKv4ScanThreads) mine += p.refs[i] > 0;
+  kv4_block_before(mine, warps, live);
+  int holes = 0, moves = 0;
+  for (int i0 = 0; i0 < n; i0 += kKv4ScanThreads) {
+    const int i = i0 + tid;
+    const bool on = i < n && p.refs[i] > 0;
+    const bool hole = i < n && i < live && !on, move = on && i >= live;
+    int sum;
+    const int h = holes + kv4_block_before(hole, warps, sum);
+    holes += sum;
+    const int m = moves + kv4_block_before(move, warps, sum);
+    moves += sum;
+    if (hole) p.dst[h] = i;
+    if (move) p.src[m] = i;
+    if (i < n) {
+      p.to[i] = on && i < live ? i : -1;
+      p.refs_out[i] = on && i < live ? p.refs[i] : 0;
+    }
+  }
+  __syncthreads();  // one CTA: its own global writes above are visible to it
+  for (int k = tid; k < moves; k += kKv4ScanThreads) {
+    p.to[p.src[k]] = p.dst[k];
+    p.refs_out[p.dst[k]] = p.refs[p.src[k]];
+  }
+  if (tid == 0) {
+    p.info[0] = live;
+    p.info[1] = moves;
+    p.info[2] = p.info[3] = 0;
+  }
+}
+
+// The table's entries and the pages' bytes: CTAs share the entries, then the (move, layer) pairs.
+__global__ void __launch_bounds__(kKv4CopyThreads) kv4_compact_move_kernel(const Kv4CompactParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const size_t n = static_cast<size_t>(p.batch) * p.max_pages;
+  for (size_t i = static_cast<size_t>(blockIdx.x) * kKv4CopyThreads + threadIdx.x; i < n;
+       i += static_cast<size_t>(gridDim.x) * kKv4CopyThreads) {
+    const int id = p.table[i];
+    p.table_out[i] = id >= 0 && id < p.data.n_pages ? p.to[id] : -1;
+  }
+  const long long work = static_cast<long long>(p.info[1]) * p.data.layers;
+  for (long long w = blockIdx.x; w < work; w += gridDim.x) {
+    const int k = static_cast<int>(w / p.data.layers);
+    kv4_copy_page(p.data, static_cast<int>(w % p.data.layers), p.src[k], p.dst[k], 0, 1);
+  }
+}
+
+}  // namespace b2

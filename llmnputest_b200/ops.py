@@ -7,6 +7,7 @@ kernels do not support -- there is no eager or CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -590,3 +591,314 @@ def gated_attn_decode(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor
                  _ptr(pos), bsz, n_q_heads, n_kv_heads, d, ctx_max, max_len, float(eps), _ptr(out), out.stride(0),
                  GATED_OUT_F32 if out_f32 else 0, wp, wn, _stream())
     return out
+
+
+# ---- the 4-bit paged KV cache (b2_kv4_*)
+
+KV4_NO_ROPE = 1
+KV4_OUT_F32 = 2
+KV4_ROWS_F32 = 4
+KV4_CELL_BYTES = 1152  # 16 tokens x 64 dims of K and V
+
+
+def kv4_page_bytes(page: int, head_dim: int) -> int:
+    """Bytes of one kv head's part of a page (the last dim of a pool)."""
+    if page < 16 or page % 16 or head_dim not in (64, 128, 256):
+        raise ValueError("page must be a multiple of 16, head_dim 64, 128 or 256")
+    return page // 16 * (head_dim // 64) * KV4_CELL_BYTES
+
+
+def _kv4_page(page_bytes: int, head_dim: int) -> int:
+    """The page length of a pool whose last dim is page_bytes."""
+    if head_dim not in (64, 128, 256):
+        raise ValueError("head_dim must be 64, 128 or 256")
+    tiles, rest = divmod(page_bytes, head_dim // 64 * KV4_CELL_BYTES)
+    if rest or not tiles:
+        raise ValueError(f"pool: a last dim of {page_bytes} bytes is no whole number of 16-token tiles")
+    return 16 * tiles
+
+
+def _kv4_need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple | None = None) -> None:
+    _need(t, name, dtype)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have the shape {shape}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _kv4_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, width: int) -> int:
+    """The row stride of [rows, >= width] with unit column stride."""
+    _need(t, name, dtype)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+    if t.dim() != 2 or t.shape[1] < width or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be [rows, >= {width}] with unit column stride, got {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], width)
+
+
+def _kv4_table(table: torch.Tensor, pos: torch.Tensor, device: torch.device) -> tuple[int, int]:
+    _need(table, "table", torch.int32)
+    if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
+        raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
+    _kv4_need(table, "table", torch.int32, device)
+    _kv4_need(pos, "pos", torch.int32, device, (table.shape[0],))
+    return table.shape[0], table.shape[1]
+
+
+def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> int:
+    _need(pool, "pool", torch.uint8)
+    if pool.dim() != 3 or pool.shape[1] != n_kv_heads or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous [n_pages, {n_kv_heads}, page bytes], got {tuple(pool.shape)}")
+    return _kv4_page(pool.shape[2], head_dim)
+
+
+def _kv4_call(device: torch.device, name: str, *args) -> None:
+    """A call on `device`'s current stream, whichever device is current."""
+    if torch.cuda.current_device() == device.index:
+        _native.call(name, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            _native.call(name, *args, _stream())
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_ws_bytes(device: int, name: str, *args) -> int:
+    with torch.cuda.device(device):
+        n = ctypes.c_size_t(0)
+        _native.call(name, *args, ctypes.byref(n))
+    return n.value
+
+
+def _kv4_ws(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor | None:
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _kv4_need(workspace, "workspace", torch.uint8, device)
+    if workspace.numel() < need or workspace.data_ptr() % 16:
+        raise ValueError(f"workspace must hold {need} bytes, 16-byte aligned")
+    return workspace
+
+
+def _opt(t: torch.Tensor | None) -> ctypes.c_void_p | None:
+    return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _kv4_cu(cu: torch.Tensor | None, batch: int, rows: int, device: torch.device) -> None:
+    if cu is not None:
+        _kv4_need(cu, "cu", torch.int32, device, (batch + 1,))
+    elif rows != batch:
+        raise ValueError(f"{rows} rows for {batch} sequences: pass the row offsets cu")
+
+
+def _kv4_summary(summary: torch.Tensor | None, pool: torch.Tensor, head_dim: int) -> None:
+    if summary is not None:
+        _kv4_need(summary, "summary", torch.bfloat16, pool.device, (*pool.shape[:-1], 2, head_dim))
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *,
+               n_kv_heads: int, head_dim: int, cu: torch.Tensor | None = None, theta: float | None = 10000.0,
+               summary: torch.Tensor | None = None) -> None:
+    """Quantise new rows into the 4-bit paged cache, in place (see b2_kv4_append).
+
+    k, v [rows, >= Hkv*D] fp32 or bf16 (slices of one projection's output are accepted);
+    pool uint8 [n_pages, Hkv, kv4_page_bytes(page, D)]; table int32 [B, max_pages]; pos
+    int32 [B], the position of each sequence's first new row (-1: none); cu int32 [B + 1]
+    row offsets (None: one row per sequence); theta None: keys are stored as given; summary
+    bf16 [n_pages, Hkv, 2, D] takes the new keys in (for kv4_select)."""
+    page = _kv4_pool(pool, n_kv_heads, head_dim)
+    dev = pool.device
+    batch, max_pages = _kv4_table(table, pos, dev)
+    if k.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("k must be fp32 or bf16")
+    ld_k = _kv4_rows(k, "k", k.dtype, dev, n_kv_heads * head_dim)
+    ld_v = _kv4_rows(v, "v", k.dtype, dev, n_kv_heads * head_dim)
+    rows = k.shape[0]
+    if v.shape[0] != rows:
+        raise ValueError("k and v have different numbers of rows")
+    _kv4_cu(cu, batch, rows, dev)
+    _kv4_summary(summary, pool, head_dim)
+    flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_ROWS_F32 if k.dtype == torch.float32 else 0)
+    _kv4_call(dev, "b2_kv4_append", _ptr(k), _ptr(v), ld_k, ld_v, rows, _ptr(pool), _ptr(table), _ptr(pos), _opt(cu),
+              _opt(summary), batch, n_kv_heads, head_dim, page, max_pages, pool.shape[0], float(theta or 0.0), flags)
+
+
+def kv4_gather(pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, rows: int, *, n_kv_heads: int,
+               head_dim: int, cu: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Read rows of the 4-bit paged cache back as k, v [rows, Hkv*D] (see b2_kv4_gather).
+
+    Sequence b's tokens pos[b], pos[b] + 1, ... go to rows cu[b] .. cu[b+1] - 1 (cu None:
+    one token per sequence).  dtype bf16 or fp32.  Rows that no token goes to keep what
+    `out` holds; without `out` they are not set."""
+    page = _kv4_pool(pool, n_kv_heads, head_dim)
+    dev, width = pool.device, n_kv_heads * head_dim
+    batch, max_pages = _kv4_table(table, pos, dev)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("dtype must be fp32 or bf16")
+    _kv4_cu(cu, batch, rows, dev)
+    k, v = out if out is not None else torch.empty((2, rows, width), dtype=dtype, device=dev).unbind(0)
+    ld_k, ld_v = _kv4_rows(k, "out k", dtype, dev, width), _kv4_rows(v, "out v", dtype, dev, width)
+    if k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError(f"out must have {rows} rows")
+    _kv4_call(dev, "b2_kv4_gather", _ptr(k), _ptr(v), ld_k, ld_v, rows, _ptr(pool), _ptr(table), _ptr(pos), _opt(cu),
+              batch, n_kv_heads, head_dim, page, max_pages, pool.shape[0],
+              KV4_ROWS_F32 if dtype == torch.float32 else 0)
+    return k, v
+
+
+def kv4_decode_workspace_bytes(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, page: int, max_len: int,
+                               n_sel: int = 0) -> int:
+    """Workspace of kv4_decode on the current device (0 when nothing is split)."""
+    return _kv4_ws_bytes(torch.cuda.current_device(), "b2_kv4_decode_workspace_size", batch, n_q_heads, n_kv_heads,
+                         head_dim, page, n_sel, max_len)
+
+
+def kv4_decode(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *, n_q_heads: int,
+               n_kv_heads: int, head_dim: int, theta: float | None = 10000.0, scale: float | None = None,
+               max_len: int | None = None, select: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               out_f32: bool = False, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention over the 4-bit paged cache, one query per sequence (see b2_kv4_decode).
+
+    q fp32 [B, >= Hq*D], rotated to pos unless theta is None; pool, table and pos as
+    kv4_append takes them, the tokens 0..pos appended before (pos -1: the row becomes
+    zeros).  select int32 [B, Hkv, n_sel] (kv4_select): attend to those pages alone.
+    max_len (default: the table's) bounds pos + 1 and sizes the split.  Returns [B, Hq*D]
+    bf16, or fp32 with out_f32."""
+    page = _kv4_pool(pool, n_kv_heads, head_dim)
+    dev, width = pool.device, n_q_heads * head_dim
+    batch, max_pages = _kv4_table(table, pos, dev)
+    ld_q = _kv4_rows(q, "q", torch.float32, dev, width)
+    odt = torch.float32 if out_f32 else torch.bfloat16
+    if out is None:
+        out = torch.empty((batch, width), dtype=odt, device=dev)
+    ldo = _kv4_rows(out, "out", odt, dev, width)
+    if q.shape[0] != batch or out.shape[0] != batch:
+        raise ValueError(f"q and out must have {batch} rows")
+    n_sel = 0
+    if select is not None:
+        _need(select, "select", torch.int32)
+        if select.dim() != 3 or select.shape[:2] != (batch, n_kv_heads) or not select.shape[2]:
+            raise ValueError(f"select must be [{batch}, {n_kv_heads}, n_sel], got {tuple(select.shape)}")
+        _kv4_need(select, "select", torch.int32, dev)
+        n_sel = select.shape[2]
+    max_len = max_pages * page if max_len is None else max_len
+    need = _kv4_ws_bytes(dev.index, "b2_kv4_decode_workspace_size", batch, n_q_heads, n_kv_heads, head_dim, page,
+                         n_sel, max_len)
+    ws = _kv4_ws(workspace, need, dev)
+    flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_OUT_F32 if out_f32 else 0)
+    _kv4_call(dev, "b2_kv4_decode", _ptr(q), ld_q, _ptr(pool), _ptr(table), _ptr(pos), _opt(select), n_sel, batch,
+              n_q_heads, n_kv_heads, head_dim, page, max_pages, pool.shape[0], max_len, float(theta or 0.0),
+              float(head_dim ** -0.5 if scale is None else scale), _ptr(out), ldo, _opt(ws),
+              ws.numel() if ws is not None else 0, flags)
+    return out
+
+
+def kv4_select_workspace_bytes(batch: int, n_kv_heads: int, page: int, max_len: int) -> int:
+    """Workspace of kv4_select."""
+    return _kv4_ws_bytes(torch.cuda.current_device(), "b2_kv4_select_workspace_size", batch, n_kv_heads, page, max_len)
+
+
+def kv4_select(q: torch.Tensor, summary: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *, n_q_heads: int,
+               n_kv_heads: int, head_dim: int, page: int, n_sel: int, theta: float | None = 10000.0,
+               max_len: int | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The n_sel pages each kv head of each query attends to in a long cache, for
+    kv4_decode's select (see b2_kv4_select): int32 [B, Hkv, n_sel] page indices, ascending,
+    -1 behind them.
+
+    q and theta as kv4_decode takes them; summary bf16 [n_pages, Hkv, 2, D] as kv4_append
+    keeps it; page the pool's page length."""
+    _need(summary, "summary", torch.bfloat16)
+    dev = summary.device
+    _kv4_need(summary, "summary", torch.bfloat16, dev, (summary.shape[0], n_kv_heads, 2, head_dim))
+    batch, max_pages = _kv4_table(table, pos, dev)
+    ld_q = _kv4_rows(q, "q", torch.float32, dev, n_q_heads * head_dim)
+    if q.shape[0] != batch:
+        raise ValueError(f"q must have {batch} rows")
+    if n_sel < 1:
+        raise ValueError("n_sel must be >= 1")
+    if out is None:
+        out = torch.empty((batch, n_kv_heads, n_sel), dtype=torch.int32, device=dev)
+    _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
+    max_len = max_pages * page if max_len is None else max_len
+    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_select_workspace_size", batch, n_kv_heads, page, max_len),
+                 dev)
+    _kv4_call(dev, "b2_kv4_select", _ptr(q), ld_q, _ptr(summary), _ptr(table), _ptr(pos), _ptr(out), n_sel, batch,
+              n_q_heads, n_kv_heads, head_dim, page, max_pages, summary.shape[0], max_len, float(theta or 0.0),
+              _ptr(ws), ws.numel(), KV4_NO_ROPE if theta is None else 0)
+    return out
+
+
+def _kv4_layers(pool: torch.Tensor, summary: torch.Tensor | None) -> tuple:
+    """The arguments for a cache's pages: pool [layers, n_pages, Hkv, bytes], summary
+    [layers, n_pages, Hkv, 2, D] or None."""
+    _need(pool, "pool", torch.uint8)
+    if pool.dim() != 4 or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous [layers, n_pages, Hkv, page bytes], got {tuple(pool.shape)}")
+    if summary is not None:
+        _need(summary, "summary", torch.bfloat16)
+        if summary.dim() != 5 or summary.shape[:3] != pool.shape[:3]:
+            raise ValueError(f"summary must be [layers, n_pages, Hkv, 2, D] beside the pool, got {tuple(summary.shape)}")
+        _kv4_need(summary, "summary", torch.bfloat16, pool.device)
+    return (_ptr(pool), pool.shape[2] * pool.shape[3], _opt(summary),
+            2 * summary[0, 0].numel() if summary is not None else 0, pool.shape[0], pool.shape[1])
+
+
+def kv4_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                   summary: torch.Tensor | None = None) -> None:
+    """Copy pages src[i] to dst[i] in every layer of a cache (see b2_kv4_copy_pages): pool
+    uint8 [layers, n_pages, Hkv, page bytes], summary bf16 [layers, n_pages, Hkv, 2, D] or
+    None, src and dst int32 [n], the destinations distinct and none of them a source."""
+    args = _kv4_layers(pool, summary)
+    _need(src, "src", torch.int32)
+    if src.dim() != 1:
+        raise ValueError("src must be [n]")
+    _kv4_need(src, "src", torch.int32, pool.device)
+    _kv4_need(dst, "dst", torch.int32, pool.device, tuple(src.shape))
+    _kv4_call(pool.device, "b2_kv4_copy_pages", *args, _ptr(src), _ptr(dst), src.numel())
+
+
+def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
+                parent: torch.Tensor, *, head_dim: int, reserve: torch.Tensor | None = None,
+                summary: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> tuple:
+    """New rows of a cache's page table: row b goes on with the tokens of row parent[b] (-1:
+    with none) and has pages for reserve[b] more (see b2_kv4_reorder).  Forks, frees and
+    reserves pages; copies the last page of a row that several go on with.
+
+    pool uint8 [layers, n_pages, Hkv, page bytes]; table int32 [B, max_pages]; lens, parent,
+    reserve int32 [B]; refs int32 [n_pages].  Returns (table, lens, refs, info) anew; info
+    int32 [4]: free pages left, pages copied, pages missing, 0."""
+    args = _kv4_layers(pool, summary)
+    dev, page = pool.device, _kv4_page(pool.shape[3], head_dim)
+    batch, max_pages = _kv4_table(table, lens, dev)
+    _kv4_need(refs, "refs", torch.int32, dev, (pool.shape[1],))
+    _kv4_need(parent, "parent", torch.int32, dev, (batch,))
+    if reserve is not None:
+        _kv4_need(reserve, "reserve", torch.int32, dev, (batch,))
+    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, pool.shape[1]),
+                 dev)
+    table_out, lens_out, refs_out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
+    info = torch.empty(4, dtype=torch.int32, device=dev)
+    _kv4_call(dev, "b2_kv4_reorder", *args, _ptr(table), _ptr(lens), _ptr(refs), _ptr(parent), _opt(reserve), batch,
+              max_pages, page, _ptr(table_out), _ptr(lens_out), _ptr(refs_out), _ptr(info), _ptr(ws), ws.numel())
+    return table_out, lens_out, refs_out, info
+
+
+def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, summary: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> tuple:
+    """A cache's live pages moved to the lowest page numbers (see b2_kv4_compact).  Returns
+    (table, refs, info) anew; info int32 [4]: live pages, pages moved, 0, 0."""
+    args = _kv4_layers(pool, summary)
+    dev = pool.device
+    _kv4_need(refs, "refs", torch.int32, dev, (pool.shape[1],))
+    _need(table, "table", torch.int32)
+    if table.dim() != 2 or not table.numel():
+        raise ValueError("table must be [batch, max_pages]")
+    _kv4_need(table, "table", torch.int32, dev)
+    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", pool.shape[1]), dev)
+    table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
+    info = torch.empty(4, dtype=torch.int32, device=dev)
+    _kv4_call(dev, "b2_kv4_compact", *args, _ptr(table), _ptr(refs), table.shape[0], table.shape[1], _ptr(table_out),
+              _ptr(refs_out), _ptr(info), _ptr(ws), ws.numel())
+    return table_out, refs_out, info
