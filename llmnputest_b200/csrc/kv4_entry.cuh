@@ -2,6 +2,7 @@
 // Part of the library's one translation unit; uses its device_info, fail and cuda_fail.
 #pragma once
 
+#include <atomic>
 #include <cmath>
 
 #include "kv4_append.cuh"
@@ -53,17 +54,24 @@ const b2::Kv4Rope& kv4_rope(float theta, int head_dim, int flags) {
 }
 
 struct Kv4Launch {
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   Kv4Launch(dim3 grid, int threads, void* stream, size_t smem = 0) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    if (pdl_for(kPdlOther)) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_for(kPdlOther) ? 1 : 0;
+  }
+  void cluster(int n) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = n;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
   }
 };
 
@@ -76,20 +84,23 @@ auto kv4_by_dim(int head_dim, F f) {
 }
 
 struct Kv4DecodePlan {
-  int tiles, n_splits, split_tiles;
+  int tiles, warps, n_splits, clustered;
   size_t ws_bytes;
 };
 
-// Tiles of 16 tokens split over CTAs until there are about four per SM, no split below 8 tiles.
+// Splits until the CTAs are about four per SM, no warp below two tiles; up to 16 are joined
+// in a cluster.
 Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int tokens, int sms) {
   Kv4DecodePlan pl;
   pl.tiles = (tokens + 15) / 16;
+  pl.warps = 4;
   const long long pairs = static_cast<long long>(batch) * hkv;
-  const long long most = std::max(1, pl.tiles / 8);
-  const long long s = std::max(1LL, std::min(most, (4LL * sms + pairs - 1) / pairs));
-  pl.split_tiles = static_cast<int>((pl.tiles + s - 1) / s);
-  pl.n_splits = (pl.tiles + pl.split_tiles - 1) / pl.split_tiles;
-  pl.ws_bytes = pl.n_splits > 1 ? static_cast<size_t>(batch) * hq * pl.n_splits * (head_dim + 2) * sizeof(float) : 0;
+  const long long most = std::max(1, pl.tiles / (2 * pl.warps));
+  long long s = std::max(1LL, std::min(most, (4LL * sms + pairs - 1) / pairs));
+  if (s > 16 && 16 * pairs >= sms) s = 16;
+  pl.n_splits = static_cast<int>(s);
+  pl.clustered = s > 1 && s <= 16;
+  pl.ws_bytes = s > 16 ? static_cast<size_t>(batch) * hq * pl.n_splits * (head_dim + 2) * sizeof(float) : 0;
   return pl;
 }
 
@@ -236,16 +247,29 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
   p.n_pages = n_pages;
   p.n_sel = n_sel;
   p.n_splits = pl.n_splits;
-  p.split_tiles = pl.split_tiles;
+  p.clustered = pl.clustered;
   p.max_tiles = pl.tiles;
   p.out_f32 = (flags & B2_KV4_OUT_F32) ? 1 : 0;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
-  Kv4Launch l(dim3(pl.n_splits, n_kv_heads, batch), b2::kKv4DecodeWarps * 32, stream);
   cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
-    return cudaLaunchKernelEx(&l.cfg, b2::kv4_decode_kernel<decltype(d)::value>, p, rope);
+    constexpr int D = decltype(d)::value;
+    auto kernel = b2::kv4_decode_kernel<D, 4>;
+    constexpr size_t smem = b2::kv4_decode_smem<D, 4>();
+    static std::atomic<unsigned long long> ready{0};  // devices on which the kernel's attributes are set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(ready.load() >> dev & 1)) {
+      cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (r == cudaSuccess) r = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (r != cudaSuccess) return r;
+      ready.fetch_or(1ull << dev);
+    }
+    Kv4Launch l(dim3(pl.n_splits, n_kv_heads, batch), pl.warps * 32, stream, smem);
+    if (pl.clustered) l.cluster(pl.n_splits);
+    return cudaLaunchKernelEx(&l.cfg, kernel, p, rope);
   });
   if (e != cudaSuccess) return cuda_fail(e, "kv4 decode launch");
-  if (pl.n_splits > 1) {
+  if (pl.ws_bytes) {
     Kv4Launch c(dim3(n_q_heads, batch, 1), head_dim, stream);
     e = kv4_by_dim(head_dim, [&](auto d) {
       return cudaLaunchKernelEx(&c.cfg, b2::kv4_combine_kernel<decltype(d)::value>, p);

@@ -618,52 +618,60 @@ def _kv4_page(page_bytes: int, head_dim: int) -> int:
     return 16 * tiles
 
 
-def _kv4_need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple | None = None) -> None:
+def _kv4_need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple | None = None) -> int:
+    """A contiguous device tensor's address; the checks are one expression, as a decode
+    step makes some thirty of them, and only a failed one is looked into."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.is_contiguous()
+            and (shape is None or t.shape == shape)):
+        return t.data_ptr()
     _need(t, name, dtype)
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the pool on {device}")
     if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have the shape {shape}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _kv4_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, width: int) -> int:
+def _kv4_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, rows: int, width: int) -> int:
     """The row stride of [rows, >= width] with unit column stride."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.dim() == 2:
+        (n, w), (ld, unit) = t.shape, t.stride()
+        if n == rows and w >= width and (unit == 1 or w == 1):
+            return ld if n > 1 else w
     _need(t, name, dtype)
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the pool on {device}")
-    if t.dim() != 2 or t.shape[1] < width or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{name} must be [rows, >= {width}] with unit column stride, got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], width)
+    raise ValueError(f"{name} must be [{rows}, >= {width}] with unit column stride, got {tuple(t.shape)}")
 
 
-def _kv4_table(table: torch.Tensor, pos: torch.Tensor, device: torch.device) -> tuple[int, int]:
-    _need(table, "table", torch.int32)
-    if table.dim() != 2 or not table.shape[0] or not table.shape[1]:
-        raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
+def _kv4_table(table: torch.Tensor, device: torch.device) -> torch.Size:
+    """[batch, max_pages] of a page table."""
     _kv4_need(table, "table", torch.int32, device)
-    _kv4_need(pos, "pos", torch.int32, device, (table.shape[0],))
-    return table.shape[0], table.shape[1]
+    if table.dim() != 2 or not table.numel():
+        raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
+    return table.shape
 
 
-def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> int:
+def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> tuple[int, int]:
+    """(pages, page length) of one layer's pool."""
     _need(pool, "pool", torch.uint8)
     if pool.dim() != 3 or pool.shape[1] != n_kv_heads or not pool.is_contiguous():
         raise ValueError(f"pool must be contiguous [n_pages, {n_kv_heads}, page bytes], got {tuple(pool.shape)}")
-    return _kv4_page(pool.shape[2], head_dim)
+    return pool.shape[0], _kv4_page(pool.shape[2], head_dim)
 
 
 def _kv4_call(device: torch.device, name: str, *args) -> None:
     """A call on `device`'s current stream, whichever device is current."""
-    if torch.cuda.current_device() == device.index:
-        _native.call(name, *args, _stream())
-    else:
+    index = device.index
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
-            _native.call(name, *args, _stream())
+            return _kv4_call(device, name, *args)
+    status = getattr(_native.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _native.check(status, name)
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def _kv4_ws_bytes(device: int, name: str, *args) -> int:
     with torch.cuda.device(device):
         n = ctypes.c_size_t(0)
@@ -674,26 +682,17 @@ def _kv4_ws_bytes(device: int, name: str, *args) -> int:
 def _kv4_ws(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor | None:
     if workspace is None:
         return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _kv4_need(workspace, "workspace", torch.uint8, device)
-    if workspace.numel() < need or workspace.data_ptr() % 16:
+    if _kv4_need(workspace, "workspace", torch.uint8, device) % 16 or workspace.numel() < need:
         raise ValueError(f"workspace must hold {need} bytes, 16-byte aligned")
     return workspace
 
 
-def _opt(t: torch.Tensor | None) -> ctypes.c_void_p | None:
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
-
-
-def _kv4_cu(cu: torch.Tensor | None, batch: int, rows: int, device: torch.device) -> None:
+def _kv4_cu(cu: torch.Tensor | None, batch: int, rows: int, device: torch.device) -> int | None:
     if cu is not None:
-        _kv4_need(cu, "cu", torch.int32, device, (batch + 1,))
-    elif rows != batch:
+        return _kv4_need(cu, "cu", torch.int32, device, (batch + 1,))
+    if rows != batch:
         raise ValueError(f"{rows} rows for {batch} sequences: pass the row offsets cu")
-
-
-def _kv4_summary(summary: torch.Tensor | None, pool: torch.Tensor, head_dim: int) -> None:
-    if summary is not None:
-        _kv4_need(summary, "summary", torch.bfloat16, pool.device, (*pool.shape[:-1], 2, head_dim))
+    return None
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *,
@@ -706,21 +705,20 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torc
     int32 [B], the position of each sequence's first new row (-1: none); cu int32 [B + 1]
     row offsets (None: one row per sequence); theta None: keys are stored as given; summary
     bf16 [n_pages, Hkv, 2, D] takes the new keys in (for kv4_select)."""
-    page = _kv4_pool(pool, n_kv_heads, head_dim)
-    dev = pool.device
-    batch, max_pages = _kv4_table(table, pos, dev)
-    if k.dtype not in (torch.float32, torch.bfloat16):
+    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
+    dev, dtype, rows = pool.device, k.dtype, k.shape[0]
+    batch, max_pages = _kv4_table(table, dev)
+    if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("k must be fp32 or bf16")
-    ld_k = _kv4_rows(k, "k", k.dtype, dev, n_kv_heads * head_dim)
-    ld_v = _kv4_rows(v, "v", k.dtype, dev, n_kv_heads * head_dim)
-    rows = k.shape[0]
-    if v.shape[0] != rows:
-        raise ValueError("k and v have different numbers of rows")
-    _kv4_cu(cu, batch, rows, dev)
-    _kv4_summary(summary, pool, head_dim)
-    flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_ROWS_F32 if k.dtype == torch.float32 else 0)
-    _kv4_call(dev, "b2_kv4_append", _ptr(k), _ptr(v), ld_k, ld_v, rows, _ptr(pool), _ptr(table), _ptr(pos), _opt(cu),
-              _opt(summary), batch, n_kv_heads, head_dim, page, max_pages, pool.shape[0], float(theta or 0.0), flags)
+    ld_k = _kv4_rows(k, "k", dtype, dev, rows, n_kv_heads * head_dim)
+    ld_v = _kv4_rows(v, "v", dtype, dev, rows, n_kv_heads * head_dim)
+    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
+    offsets = _kv4_cu(cu, batch, rows, dev)
+    near = (None if summary is None else
+            _kv4_need(summary, "summary", torch.bfloat16, dev, (n_pages, n_kv_heads, 2, head_dim)))
+    flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_ROWS_F32 if dtype is torch.float32 else 0)
+    _kv4_call(dev, "b2_kv4_append", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), table.data_ptr(),
+              at, offsets, near, batch, n_kv_heads, head_dim, page, max_pages, n_pages, theta or 0.0, flags)
 
 
 def kv4_gather(pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, rows: int, *, n_kv_heads: int,
@@ -731,19 +729,19 @@ def kv4_gather(pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, rows:
     Sequence b's tokens pos[b], pos[b] + 1, ... go to rows cu[b] .. cu[b+1] - 1 (cu None:
     one token per sequence).  dtype bf16 or fp32.  Rows that no token goes to keep what
     `out` holds; without `out` they are not set."""
-    page = _kv4_pool(pool, n_kv_heads, head_dim)
+    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
     dev, width = pool.device, n_kv_heads * head_dim
-    batch, max_pages = _kv4_table(table, pos, dev)
+    batch, max_pages = _kv4_table(table, dev)
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("dtype must be fp32 or bf16")
-    _kv4_cu(cu, batch, rows, dev)
+    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
+    offsets = _kv4_cu(cu, batch, rows, dev)
     k, v = out if out is not None else torch.empty((2, rows, width), dtype=dtype, device=dev).unbind(0)
-    ld_k, ld_v = _kv4_rows(k, "out k", dtype, dev, width), _kv4_rows(v, "out v", dtype, dev, width)
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError(f"out must have {rows} rows")
-    _kv4_call(dev, "b2_kv4_gather", _ptr(k), _ptr(v), ld_k, ld_v, rows, _ptr(pool), _ptr(table), _ptr(pos), _opt(cu),
-              batch, n_kv_heads, head_dim, page, max_pages, pool.shape[0],
-              KV4_ROWS_F32 if dtype == torch.float32 else 0)
+    ld_k = _kv4_rows(k, "out k", dtype, dev, rows, width)
+    ld_v = _kv4_rows(v, "out v", dtype, dev, rows, width)
+    _kv4_call(dev, "b2_kv4_gather", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), table.data_ptr(), at,
+              offsets, batch, n_kv_heads, head_dim, page, max_pages, n_pages,
+              KV4_ROWS_F32 if dtype is torch.float32 else 0)
     return k, v
 
 
@@ -765,32 +763,32 @@ def kv4_decode(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: to
     zeros).  select int32 [B, Hkv, n_sel] (kv4_select): attend to those pages alone.
     max_len (default: the table's) bounds pos + 1 and sizes the split.  Returns [B, Hq*D]
     bf16, or fp32 with out_f32."""
-    page = _kv4_pool(pool, n_kv_heads, head_dim)
+    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
     dev, width = pool.device, n_q_heads * head_dim
-    batch, max_pages = _kv4_table(table, pos, dev)
-    ld_q = _kv4_rows(q, "q", torch.float32, dev, width)
+    batch, max_pages = _kv4_table(table, dev)
+    ld_q = _kv4_rows(q, "q", torch.float32, dev, batch, width)
+    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     odt = torch.float32 if out_f32 else torch.bfloat16
     if out is None:
         out = torch.empty((batch, width), dtype=odt, device=dev)
-    ldo = _kv4_rows(out, "out", odt, dev, width)
-    if q.shape[0] != batch or out.shape[0] != batch:
-        raise ValueError(f"q and out must have {batch} rows")
-    n_sel = 0
+    ldo = _kv4_rows(out, "out", odt, dev, batch, width)
+    chosen, n_sel = None, 0
     if select is not None:
         _need(select, "select", torch.int32)
-        if select.dim() != 3 or select.shape[:2] != (batch, n_kv_heads) or not select.shape[2]:
+        if select.dim() != 3 or not select.shape[2]:
             raise ValueError(f"select must be [{batch}, {n_kv_heads}, n_sel], got {tuple(select.shape)}")
-        _kv4_need(select, "select", torch.int32, dev)
         n_sel = select.shape[2]
-    max_len = max_pages * page if max_len is None else max_len
+        chosen = _kv4_need(select, "select", torch.int32, dev, (batch, n_kv_heads, n_sel))
+    if max_len is None:
+        max_len = max_pages * page
     need = _kv4_ws_bytes(dev.index, "b2_kv4_decode_workspace_size", batch, n_q_heads, n_kv_heads, head_dim, page,
                          n_sel, max_len)
     ws = _kv4_ws(workspace, need, dev)
     flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_OUT_F32 if out_f32 else 0)
-    _kv4_call(dev, "b2_kv4_decode", _ptr(q), ld_q, _ptr(pool), _ptr(table), _ptr(pos), _opt(select), n_sel, batch,
-              n_q_heads, n_kv_heads, head_dim, page, max_pages, pool.shape[0], max_len, float(theta or 0.0),
-              float(head_dim ** -0.5 if scale is None else scale), _ptr(out), ldo, _opt(ws),
-              ws.numel() if ws is not None else 0, flags)
+    _kv4_call(dev, "b2_kv4_decode", q.data_ptr(), ld_q, pool.data_ptr(), table.data_ptr(), at, chosen, n_sel, batch,
+              n_q_heads, n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0,
+              head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
+              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), flags)
     return out
 
 
@@ -810,23 +808,23 @@ def kv4_select(q: torch.Tensor, summary: torch.Tensor, table: torch.Tensor, pos:
     q and theta as kv4_decode takes them; summary bf16 [n_pages, Hkv, 2, D] as kv4_append
     keeps it; page the pool's page length."""
     _need(summary, "summary", torch.bfloat16)
-    dev = summary.device
-    _kv4_need(summary, "summary", torch.bfloat16, dev, (summary.shape[0], n_kv_heads, 2, head_dim))
-    batch, max_pages = _kv4_table(table, pos, dev)
-    ld_q = _kv4_rows(q, "q", torch.float32, dev, n_q_heads * head_dim)
-    if q.shape[0] != batch:
-        raise ValueError(f"q must have {batch} rows")
+    dev, n_pages = summary.device, summary.shape[0]
+    near = _kv4_need(summary, "summary", torch.bfloat16, dev, (n_pages, n_kv_heads, 2, head_dim))
+    batch, max_pages = _kv4_table(table, dev)
+    ld_q = _kv4_rows(q, "q", torch.float32, dev, batch, n_q_heads * head_dim)
+    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     if n_sel < 1:
         raise ValueError("n_sel must be >= 1")
     if out is None:
         out = torch.empty((batch, n_kv_heads, n_sel), dtype=torch.int32, device=dev)
-    _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
-    max_len = max_pages * page if max_len is None else max_len
+    chosen = _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
+    if max_len is None:
+        max_len = max_pages * page
     ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_select_workspace_size", batch, n_kv_heads, page, max_len),
                  dev)
-    _kv4_call(dev, "b2_kv4_select", _ptr(q), ld_q, _ptr(summary), _ptr(table), _ptr(pos), _ptr(out), n_sel, batch,
-              n_q_heads, n_kv_heads, head_dim, page, max_pages, summary.shape[0], max_len, float(theta or 0.0),
-              _ptr(ws), ws.numel(), KV4_NO_ROPE if theta is None else 0)
+    _kv4_call(dev, "b2_kv4_select", q.data_ptr(), ld_q, near, table.data_ptr(), at, chosen, n_sel, batch, n_q_heads,
+              n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0, ws.data_ptr(), ws.numel(),
+              KV4_NO_ROPE if theta is None else 0)
     return out
 
 
@@ -836,13 +834,16 @@ def _kv4_layers(pool: torch.Tensor, summary: torch.Tensor | None) -> tuple:
     _need(pool, "pool", torch.uint8)
     if pool.dim() != 4 or not pool.is_contiguous():
         raise ValueError(f"pool must be contiguous [layers, n_pages, Hkv, page bytes], got {tuple(pool.shape)}")
+    layers, n_pages, hkv, nbytes = pool.shape
+    near, near_bytes = None, 0
     if summary is not None:
         _need(summary, "summary", torch.bfloat16)
-        if summary.dim() != 5 or summary.shape[:3] != pool.shape[:3]:
-            raise ValueError(f"summary must be [layers, n_pages, Hkv, 2, D] beside the pool, got {tuple(summary.shape)}")
-        _kv4_need(summary, "summary", torch.bfloat16, pool.device)
-    return (_ptr(pool), pool.shape[2] * pool.shape[3], _opt(summary),
-            2 * summary[0, 0].numel() if summary is not None else 0, pool.shape[0], pool.shape[1])
+        if summary.dim() != 5:
+            raise ValueError(f"summary must be [layers, n_pages, Hkv, 2, D], got {tuple(summary.shape)}")
+        dim = summary.shape[4]
+        near = _kv4_need(summary, "summary", torch.bfloat16, pool.device, (layers, n_pages, hkv, 2, dim))
+        near_bytes = 4 * hkv * dim
+    return pool.data_ptr(), hkv * nbytes, near, near_bytes, layers, n_pages
 
 
 def kv4_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -854,9 +855,9 @@ def kv4_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     _need(src, "src", torch.int32)
     if src.dim() != 1:
         raise ValueError("src must be [n]")
-    _kv4_need(src, "src", torch.int32, pool.device)
-    _kv4_need(dst, "dst", torch.int32, pool.device, tuple(src.shape))
-    _kv4_call(pool.device, "b2_kv4_copy_pages", *args, _ptr(src), _ptr(dst), src.numel())
+    n = src.numel()
+    _kv4_call(pool.device, "b2_kv4_copy_pages", *args, _kv4_need(src, "src", torch.int32, pool.device),
+              _kv4_need(dst, "dst", torch.int32, pool.device, (n,)), n)
 
 
 def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
@@ -870,19 +871,18 @@ def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, ref
     reserve int32 [B]; refs int32 [n_pages].  Returns (table, lens, refs, info) anew; info
     int32 [4]: free pages left, pages copied, pages missing, 0."""
     args = _kv4_layers(pool, summary)
-    dev, page = pool.device, _kv4_page(pool.shape[3], head_dim)
-    batch, max_pages = _kv4_table(table, lens, dev)
-    _kv4_need(refs, "refs", torch.int32, dev, (pool.shape[1],))
-    _kv4_need(parent, "parent", torch.int32, dev, (batch,))
-    if reserve is not None:
-        _kv4_need(reserve, "reserve", torch.int32, dev, (batch,))
-    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, pool.shape[1]),
-                 dev)
-    table_out, lens_out, refs_out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
-    info = torch.empty(4, dtype=torch.int32, device=dev)
-    _kv4_call(dev, "b2_kv4_reorder", *args, _ptr(table), _ptr(lens), _ptr(refs), _ptr(parent), _opt(reserve), batch,
-              max_pages, page, _ptr(table_out), _ptr(lens_out), _ptr(refs_out), _ptr(info), _ptr(ws), ws.numel())
-    return table_out, lens_out, refs_out, info
+    dev, n_pages, page = pool.device, pool.shape[1], _kv4_page(pool.shape[3], head_dim)
+    batch, max_pages = _kv4_table(table, dev)
+    rows = (_kv4_need(lens, "lens", torch.int32, dev, (batch,)), _kv4_need(refs, "refs", torch.int32, dev, (n_pages,)),
+            _kv4_need(parent, "parent", torch.int32, dev, (batch,)),
+            None if reserve is None else _kv4_need(reserve, "reserve", torch.int32, dev, (batch,)))
+    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, n_pages), dev)
+    # the new rows are parts of one allocation
+    info, refs_out, lens_out, table_out = torch.empty(4 + n_pages + batch + batch * max_pages, dtype=torch.int32,
+                                                      device=dev).split([4, n_pages, batch, batch * max_pages])
+    _kv4_call(dev, "b2_kv4_reorder", *args, table.data_ptr(), *rows, batch, max_pages, page, table_out.data_ptr(),
+              lens_out.data_ptr(), refs_out.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel())
+    return table_out.view(batch, max_pages), lens_out, refs_out, info
 
 
 def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, summary: torch.Tensor | None = None,
@@ -890,15 +890,12 @@ def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, 
     """A cache's live pages moved to the lowest page numbers (see b2_kv4_compact).  Returns
     (table, refs, info) anew; info int32 [4]: live pages, pages moved, 0, 0."""
     args = _kv4_layers(pool, summary)
-    dev = pool.device
-    _kv4_need(refs, "refs", torch.int32, dev, (pool.shape[1],))
-    _need(table, "table", torch.int32)
-    if table.dim() != 2 or not table.numel():
-        raise ValueError("table must be [batch, max_pages]")
-    _kv4_need(table, "table", torch.int32, dev)
-    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", pool.shape[1]), dev)
-    table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
-    info = torch.empty(4, dtype=torch.int32, device=dev)
-    _kv4_call(dev, "b2_kv4_compact", *args, _ptr(table), _ptr(refs), table.shape[0], table.shape[1], _ptr(table_out),
-              _ptr(refs_out), _ptr(info), _ptr(ws), ws.numel())
-    return table_out, refs_out, info
+    dev, n_pages = pool.device, pool.shape[1]
+    batch, max_pages = _kv4_table(table, dev)
+    held = _kv4_need(refs, "refs", torch.int32, dev, (n_pages,))
+    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", n_pages), dev)
+    info, refs_out, table_out = torch.empty(4 + n_pages + batch * max_pages, dtype=torch.int32,
+                                            device=dev).split([4, n_pages, batch * max_pages])
+    _kv4_call(dev, "b2_kv4_compact", *args, table.data_ptr(), held, batch, max_pages, table_out.data_ptr(),
+              refs_out.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel())
+    return table_out.view(batch, max_pages), refs_out, info
