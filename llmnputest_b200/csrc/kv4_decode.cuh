@@ -5,10 +5,12 @@
 //     s[t] = scale * (d (q . n) + m sum(q)),   p = softmax(s),
 //     out  = sum_t (p[t] e[t]) c[t] + sum_t p[t] f[t]
 //
-// The codes enter mma.sync m16n8k16 as they are: a nibble in the low bits of an fp16 is the
-// subnormal n * 2^-24 (or n * 2^-20 four bits up), exact, so a word of 8 codes becomes four
-// A registers with one shift and four ANDs, no conversion and no offset to take off again;
-// the scales multiply the products' fp32 sums.  S^T = K Q^T (16 tokens x 8 heads per
+// The codes enter mma.sync m16n8k16 as they are: an integer below 2^10 in the low bits of an
+// fp16 is the subnormal n * 2^-24, exact.  A byte of two codes a + 16 b goes in twice, whole
+// and as its low nibble a: two byte permutations and two ANDs make four A registers of a word
+// of 8 codes, without a conversion or an offset.  For the scores a q_a + b q_b is
+// (a + 16 b) (q_b / 16) + a (q_a - q_b / 16); of the values' sums, sum w b is
+// (sum w (a + 16 b) - sum w a) / 16 at the end.  The scales multiply the products' fp32 sums.  S^T = K Q^T (16 tokens x 8 heads per
 // instruction), O^T = V^T P^T; P moves from the accumulator's layout to the B operand's
 // with movmatrix.
 //
@@ -25,6 +27,9 @@ namespace b2 {
 
 constexpr int kKv4MaxGroup = 8;  // q heads per kv head: the N of the MMA
 
+// a CTA's sums of one pair: o [grp][D], R [grp], L [grp], up to 16 bytes
+__host__ __device__ constexpr int kv4_part_floats(int grp, int D) { return (grp * (D + 2) + 3) / 4 * 4; }
+
 struct Kv4DecodeParams {
   const float* q;  // [batch][ld_q], head j at j * D
   long long ld_q;
@@ -33,12 +38,13 @@ struct Kv4DecodeParams {
   const int* pos;    // [batch], -1: nothing to attend
   const int* sel;    // [batch][hkv][n_sel] page indices, ascending, or null
   void* out;         // [batch][ldo]
-  float* part;       // [batch][hkv][n_splits] x (o [grp][D], R [grp], L [grp]) of splits not clustered
+  float* part;       // [grid][2][kv4_part_floats]: the ends of pairs that several CTAs share
   long long ldo;
   float scale_log2;
   int batch, hq, hkv, page, max_pages, n_pages, n_sel;
-  int n_splits, clustered;  // CTAs per (sequence, kv head); joined in a cluster or through part
-  int max_tiles;            // tiles of the longest sequence planned for
+  int max_tiles;  // tiles of the longest sequence planned for
+  int splits;     // CTAs of a (sequence, kv head), a cluster; 0: the tiles are dealt over the grid
+  int2* spans;    // [batch][hkv] the CTAs that share a pair, or x = -1 (dealt over the grid)
   int out_f32;
 };
 
@@ -52,86 +58,118 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The query heads of one (sequence, kv head), ready as B operands: fp16 of q * scale * log2 e *
-// 2^-ex (the head's largest in [1, 2)), odd dims / 16 to meet the nibbles four bits up.
+// The query heads of one (sequence, kv head), ready as B operands: of q * scale * log2 e *
+// 2^-ex (the head's largest in [1, 2)), h1 = fp16(odd dim) / 16 and h0 = fp16(even dim - h1).
+// Fragment (g, ks) of lane (head, c), with o = 16 c + 4 ks: h1 of (o + 1, o + 3), then h0 of
+// (o, o + 2).
 template <int D>
 struct Kv4Query {
   static constexpr int G = D / kKv4Group;
-  uint32_t b[G][4][2][32];          // B fragments by lane
-  float sum[G][kKv4MaxGroup];       // sum of the fp16 q over the group, * 2^-24
-  float unit[kKv4MaxGroup];         // 2^24 * 2^ex
-  __half h[kKv4MaxGroup][D];
+  __half b[G][4][2][32][2];
+  float sum[G][kKv4MaxGroup];  // sum over the group of q as the fragments have it, * 2^-24
+  float unit[kKv4MaxGroup];    // 2^24 * 2^ex
 };
 
-template <int D, int THREADS>
-__device__ __forceinline__ void kv4_load_query(const Kv4DecodeParams& p, const Kv4Rope& rope, int b, int kvh, int pos,
-                                               Kv4Query<D>& Q) {
-  constexpr int G = D / kKv4Group, J = D / 32, W = THREADS / 32;
+// A warp's heads of the query as they are stored (warp, warp + W, ..), dims lane + 32 i.
+template <int D, int W>
+struct Kv4RawQuery {
+  static constexpr int H = kKv4MaxGroup / W;
+  float x[H][D / 32];
+};
+template <int D, int W>
+__device__ __forceinline__ void kv4_load_query(const Kv4DecodeParams& p, int b, int kvh, Kv4RawQuery<D, W>& q) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = p.hq / p.hkv;
-  for (int j = warp; j < kKv4MaxGroup; j += W) {
-    float x[J];
+#pragma unroll
+  for (int h = 0; h < Kv4RawQuery<D, W>::H; ++h) {
+    const int j = warp + h * W;
     const float* src = p.q + static_cast<size_t>(b) * p.ld_q + static_cast<size_t>(kvh * grp + j) * D + lane;
 #pragma unroll
-    for (int i = 0; i < J; ++i) x[i] = j < grp ? src[32 * i] : 0.f;
-    if (rope.on) {
+    for (int i = 0; i < D / 32; ++i) q.x[h][i] = j < grp ? src[32 * i] : 0.f;
+  }
+}
+
+// A kernel parameter's table entry by a lane's own index: through its generic address, as the
+// constant port would take the 32 lanes' indices one by one.
+__device__ __forceinline__ double kv4_turn(const Kv4Rope& rope, int i) {
+  double t;
+  asm("ld.f64 %0, [%1];" : "=d"(t) : "l"(rope.turn + i));
+  return t;
+}
+
+template <int D, int W>
+__device__ __forceinline__ void kv4_prepare_query(const Kv4DecodeParams& p, const Kv4Rope& rope, int pos,
+                                                  Kv4RawQuery<D, W>& q, Kv4Query<D>& Q) {
+  constexpr int G = D / kKv4Group, J = D / 32, H = Kv4RawQuery<D, W>::H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float top[H], s[H][G];
 #pragma unroll
-      for (int i = 0; i < J / 2; ++i) {
-        double u = static_cast<double>(pos) * rope.turn[lane + 32 * i];
-        u -= rint(u);
-        float sn, cs;
-        sincospif(2.f * static_cast<float>(u), &sn, &cs);
-        const float a = x[i], c = x[i + J / 2];
-        x[i] = a * cs - c * sn;
-        x[i + J / 2] = c * cs + a * sn;
-      }
+  for (int h = 0; h < H; ++h) top[h] = 0.f;
+#pragma unroll
+  for (int i = 0; i < J / 2; ++i) {
+    float sn = 0.f, cs = 1.f;
+    if (rope.on) {
+      double u = static_cast<double>(pos) * kv4_turn(rope, lane + 32 * i);
+      u -= rint(u);
+      sincospif(2.f * static_cast<float>(u), &sn, &cs);
     }
-    float top = 0.f;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const float a = q.x[h][i] * p.scale_log2, z = q.x[h][i + J / 2] * p.scale_log2;
+      q.x[h][i] = a * cs - z * sn;
+      q.x[h][i + J / 2] = z * cs + a * sn;
+      top[h] = fmaxf(top[h], fmaxf(fabsf(q.x[h][i]), fabsf(q.x[h][i + J / 2])));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int h = 0; h < H; ++h) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    int ex = 0;
+    if (top[h] > 0.f && top[h] < INFINITY)
+      ex = max(-100, min(100, static_cast<int>((__float_as_uint(top[h]) >> 23) & 255u) - 127));
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    const int j = warp + h * W;
 #pragma unroll
     for (int i = 0; i < J; ++i) {
-      x[i] *= p.scale_log2;
-      top = fmaxf(top, fabsf(x[i]));
-    }
-    top = warp_max(top);
-    int ex = 0;
-    if (top > 0.f && top < INFINITY) ex = max(-100, min(100, static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127));
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const __half hv = __float2half_rn(x[2 * g + e] * down);
-        s += __half2float(hv);
-        Q.h[j][64 * g + 32 * e + lane] = hv;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) Q.sum[g][j] = s * 5.9604644775390625e-8f;  // 2^-24
+      const int d = (lane + 32 * i) & 63;  // this lane's dim of the group
+      const float x = q.x[h][i] * down;
+      const float h1 = __half2float(__float2half_rn(__half2float(__float2half_rn(x)) * 0.0625f));  // for odd lanes
+      const float beside = __shfl_xor_sync(0xffffffffu, h1, 1);
+      const __half v = __float2half_rn(lane & 1 ? h1 : x - beside);
+      const float as_is = lane & 1 ? 16.f * h1 : __half2float(v) + beside;
+      s[h][i / 2] = i % 2 ? s[h][i / 2] + as_is : as_is;
+      Q.b[i / 2][d >> 2 & 3][1 - (lane & 1)][4 * j + (d >> 4)][d >> 1 & 1] = v;
     }
     if (lane == 0) Q.unit[j] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23) * 16777216.f;
   }
-  __syncthreads();
-  // fragment (g, w, sub) of k-step 2 w + sub: b0 = dims (o, o + 4), b1 = dims (o + 1, o + 5) / 16
-  // with o = 16 c + 8 w + 2 sub
-  for (int e = threadIdx.x; e < G * 4 * 32; e += THREADS) {
-    const int l = e & 31, ks = e >> 5 & 3, g = e >> 7;
-    const __half* src = &Q.h[l >> 2][64 * g + 16 * (l & 3) + 8 * (ks >> 1) + 2 * (ks & 1)];
-    const __half s16 = __float2half_rn(0.0625f);
-    const __half2 v0 = __halves2half2(src[0], src[4]), v1 = __halves2half2(__hmul(src[1], s16), __hmul(src[5], s16));
-    Q.b[g][ks][0][l] = *reinterpret_cast<const uint32_t*>(&v0);
-    Q.b[g][ks][1][l] = *reinterpret_cast<const uint32_t*>(&v1);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[h][g] += __shfl_xor_sync(0xffffffffu, s[h][g], o);
+  if (lane == 0) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int g = 0; g < G; ++g) Q.sum[g][warp + h * W] = s[h][g] * 5.9604644775390625e-8f;  // 2^-24
   }
-  __syncthreads();
 }
 
 // Running state of one warp: heads 2c and 2c + 1 of the lane.
 template <int D>
 struct Kv4State {
   static constexpr int G = D / kKv4Group;
-  float o[G][4][4];   // O^T accumulators, m-tile i of group g: dims 8g'+i and 8g'+4+i
+  float o[G][4][4];   // O^T accumulators of group g, rows 8 (lane / 4) + i and + 4: even i the sum of
+                      // w a (dim i), odd i that of w (a + 16 b) (dims i - 1 and i)
   float m[G][2];      // sum p f
   float l[2], r[2];
 };
+
+// Orders this thread's accesses to shared memory before later bulk copies into it.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 2^x, flushing what is below fp32's normal range: a weight that small is nothing beside 1
 __device__ __forceinline__ float kv4_ex2(float x) {
@@ -140,14 +178,22 @@ __device__ __forceinline__ float kv4_ex2(float x) {
   return y;
 }
 
-// NT tiles of 16 tokens; the G cells of tile n start at cell + n * stride, left[n] of its
-// tokens count.
-template <int D, int NT>
-__device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, const int (&left)[NT],
+// A B with nothing to add to.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// NT tiles of 16 tokens; the G cells of tile n start at tile0 + n * stride.  MASK: only
+// left[n] of its tokens count.
+template <int D, int NT, bool MASK>
+__device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, const int* left,
                                           const uint32_t (&qb)[D / 64][4][2], const float (&qs)[D / 64][2],
                                           const float (&unit)[2], Kv4State<D>& st) {
   constexpr int G = D / kKv4Group;
-  constexpr uint32_t kLo = 0x000F000Fu, kHi = 0x00F000F0u;
+  constexpr uint32_t kLo = 0x000F000Fu;
   const int lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
   float y[NT][4], e[NT][G][2], f[NT][G][2], emax[NT][2];
 #pragma unroll
@@ -159,14 +205,16 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
       const uint4 kw = *reinterpret_cast<const uint4*>(at + gl * 64 + c * 16);
       const uint2 km = *reinterpret_cast<const uint2*>(at + kKv4KMeta + gl * 8);
       const uint2 vm = *reinterpret_cast<const uint2*>(at + kKv4VMeta + gl * 8);
-      float a[4] = {0.f, 0.f, 0.f, 0.f};
+      float a[4];
       // words kw.x, kw.y are token gl's, kw.z, kw.w token gl + 8's
-      mma_f16_m16n8k16(a[0], a[1], a[2], a[3], kw.x & kLo, kw.z & kLo, kw.x & kHi, kw.z & kHi, qb[g][0][0], qb[g][0][1]);
-      mma_f16_m16n8k16(a[0], a[1], a[2], a[3], (kw.x >> 8) & kLo, (kw.z >> 8) & kLo, (kw.x >> 8) & kHi,
-                       (kw.z >> 8) & kHi, qb[g][1][0], qb[g][1][1]);
-      mma_f16_m16n8k16(a[0], a[1], a[2], a[3], kw.y & kLo, kw.w & kLo, kw.y & kHi, kw.w & kHi, qb[g][2][0], qb[g][2][1]);
-      mma_f16_m16n8k16(a[0], a[1], a[2], a[3], (kw.y >> 8) & kLo, (kw.w >> 8) & kLo, (kw.y >> 8) & kHi,
-                       (kw.w >> 8) & kHi, qb[g][3][0], qb[g][3][1]);
+      const uint32_t t0[2] = {kw.x, kw.y}, t1[2] = {kw.z, kw.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t sel = k & 1 ? 0x4342u : 0x4140u;  // a word's bytes 0 and 1, or 2 and 3, 16 bits each
+        const uint32_t y0 = prmt(t0[k >> 1], 0u, sel), y1 = prmt(t1[k >> 1], 0u, sel);
+        if (k == 0) mma_f16_first(a, y0, y1, y0 & kLo, y1 & kLo, qb[g][k][0], qb[g][k][1]);
+        else mma_f16_m16n8k16(a[0], a[1], a[2], a[3], y0, y1, y0 & kLo, y1 & kLo, qb[g][k][0], qb[g][k][1]);
+      }
       const float d0 = bf16lo_to_f32(km.x), m0 = bf16hi_to_f32(km.x), d1 = bf16lo_to_f32(km.y), m1 = bf16hi_to_f32(km.y);
       y[n][0] = fmaf(d0, a[0], fmaf(m0, qs[g][0], y[n][0]));
       y[n][1] = fmaf(d0, a[1], fmaf(m0, qs[g][1], y[n][1]));
@@ -177,7 +225,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
       e[n][g][1] = fmaxf(bf16lo_to_f32(vm.y), kKv4MinStep);
       f[n][g][1] = bf16hi_to_f32(vm.y);
     }
-    if (left[n] < kKv4Tile) {  // what lies behind the last token may hold anything
+    if (MASK) {  // what lies behind the last token may hold anything
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (gl + 8 * i >= left[n]) {
@@ -246,12 +294,13 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
       const uint32_t b1 = movmatrix_trans(pack_f16x2(pr[n][2] * e[n][g][1], pr[n][3] * e[n][g][1]));
       const uint4 v = *reinterpret_cast<const uint4*>(tile0 + n * stride + g * kKv4CellBytes + kKv4VCodes + gl * 64 + c * 16);
       float(&o)[4][4] = st.o[g];
-      mma_f16_m16n8k16(o[0][0], o[0][1], o[0][2], o[0][3], v.x & kLo, v.y & kLo, v.z & kLo, v.w & kLo, b0, b1);
-      mma_f16_m16n8k16(o[1][0], o[1][1], o[1][2], o[1][3], v.x & kHi, v.y & kHi, v.z & kHi, v.w & kHi, b0, b1);
-      mma_f16_m16n8k16(o[2][0], o[2][1], o[2][2], o[2][3], (v.x >> 8) & kLo, (v.y >> 8) & kLo, (v.z >> 8) & kLo,
-                       (v.w >> 8) & kLo, b0, b1);
-      mma_f16_m16n8k16(o[3][0], o[3][1], o[3][2], o[3][3], (v.x >> 8) & kHi, (v.y >> 8) & kHi, (v.z >> 8) & kHi,
-                       (v.w >> 8) & kHi, b0, b1);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // bytes 0 and 2, then 1 and 3: the same dims of two tokens
+        const uint32_t pick = k ? 0x4341u : 0x4240u;
+        const uint32_t a0 = prmt(v.x, 0u, pick), a1 = prmt(v.y, 0u, pick), a2 = prmt(v.z, 0u, pick), a3 = prmt(v.w, 0u, pick);
+        mma_f16_m16n8k16(o[2 * k][0], o[2 * k][1], o[2 * k][2], o[2 * k][3], a0 & kLo, a1 & kLo, a2 & kLo, a3 & kLo, b0, b1);
+        mma_f16_m16n8k16(o[2 * k + 1][0], o[2 * k + 1][1], o[2 * k + 1][2], o[2 * k + 1][3], a0, a1, a2, a3, b0, b1);
+      }
     }
   }
 }
@@ -262,260 +311,480 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
   else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
 }
 
-// Work split: CTA (split, kv head, sequence), W warps.  A sequence's tiles are dealt to its
-// CTAs in equal runs (by its own length, so that no CTA of a long sequence has more than its
-// share and short ones cost little), a run's stages to the warps in turn.  Every warp fills a
-// ring of its own with bulk copies, one per tile, a lane each, several stages ahead, and
-// looks the pages up 32 tiles at a time.  Splits of one (sequence, kv head) form a cluster
-// and are joined through its shared memory; more than 16 go through the workspace.
+// Work split.  A pair is a (sequence, kv head); its tiles of 16 tokens go to CTAs of W warps
+// in one of two ways.
+//   Few tiles in all: a cluster of `splits` CTAs per pair, joined through its shared memory.
+//   Else the tiles of all pairs, in a row, are dealt to as many CTAs as the GPU holds at
+//   once, the same number to each whatever the lengths: a CTA takes the end of one pair, some
+//   whole ones and the beginning of another, and a second kernel joins the pairs that were
+//   cut.  (One grid row of CTAs per pair left SMs without work at lengths of 1 to 4096, and
+//   every wave of CTAs after the first costs its start and end again.)
+// Inside a CTA the stages of a pair go to the warps in turn; a stage is 4608 bytes, or fewer
+// tiles where warps would be left without one.  Every warp fills a ring of its own with bulk
+// copies, one per tile, a lane each, and looks the pages up 32 tiles at a time.
 template <int D>
 struct Kv4Ring {
   static constexpr int G = D / kKv4Group;
   static constexpr int kTileBytes = G * kKv4CellBytes;
-  static constexpr int kTiles = D == 64 ? 2 : 1;   // tiles of a stage, taken together
-  static constexpr int kStages = D == 256 ? 3 : 4;
+  static constexpr int kTiles = 4 / G;  // tiles of a stage at most
+  static constexpr int kStages = 2;
   static constexpr int kStageBytes = kTiles * kTileBytes;
+  // what a run costs beside its tiles, in tiles of a CTA (its start and end, about 2 us)
+  static constexpr int kOverhead = 16 / G;
 };
 template <int D, int W>
 __host__ __device__ constexpr size_t kv4_decode_smem() {
   return static_cast<size_t>(W) * Kv4Ring<D>::kStages * Kv4Ring<D>::kStageBytes;
 }
 
+constexpr int kKv4MaxDealt = 1024;  // sequences of a launch whose tiles are dealt over the grid
+
+// Tiles of sequence b: 0 where it has no token, or (reported by the caller) a bad position.
+__device__ __forceinline__ int kv4_seq_tiles(const Kv4DecodeParams& p, int pos, bool& bad) {
+  bad = pos < -1 || pos >= static_cast<long long>(p.max_pages) * p.page ||
+        (!p.sel && pos >= p.max_tiles * static_cast<long long>(kKv4Tile));
+  if (bad || pos < 0) return 0;
+  return p.sel ? p.n_sel * (p.page / kKv4Tile) : pos / kKv4Tile + 1;
+}
+
+// Tiles [t_lo, t_hi) of one pair, as a CTA takes them.
+struct Kv4Run {
+  int b, kvh, pos, n_tiles, t_lo, t_hi;
+  int lg, n_stages;  // tiles of a stage: 1 << lg; this warp's stages
+};
+
 template <int D, int W>
-__global__ void __launch_bounds__(W * 32) kv4_decode_kernel(const Kv4DecodeParams p,
-                                                            const __grid_constant__ Kv4Rope rope) {
+__global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(const Kv4DecodeParams p,
+                                                                             const __grid_constant__ Kv4Rope rope) {
   using Ring = Kv4Ring<D>;
-  constexpr int G = D / kKv4Group, ST = Ring::kTiles, NS = Ring::kStages;
+  constexpr int G = D / kKv4Group, ST = Ring::kTiles, NS = Ring::kStages, NT = D == 64 ? 2 : 1;
+  constexpr int kBehind = 32;
+  constexpr int kPush = kKv4MaxGroup * D + 16;  // floats of a cluster's o that one CTA joins, over all CTAs
+  constexpr int kArea = kPush + 2 * 16 * kKv4MaxGroup > kKv4MaxDealt + 1 ? kPush + 2 * 16 * kKv4MaxGroup : kKv4MaxDealt + 1;
   extern __shared__ __align__(128) uint8_t rings[];
   __shared__ Kv4Query<D> Q;
   __shared__ __align__(8) uint64_t full[W][NS];
   __shared__ int left_s[W][NS][ST];
   __shared__ float mr[W][kKv4MaxGroup], ml[W][kKv4MaxGroup];
-  __shared__ int abort_flag;
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  __shared__ int area[kArea];  // dealt: weights of the sequences below; cluster: what the CTAs push
+  __shared__ int abort_flag, scan[W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
   const int grp = p.hq / p.hkv, tpp = p.page / kKv4Tile;
+  const size_t head_bytes = static_cast<size_t>(tpp) * Ring::kTileBytes;
+  const uint64_t once = l2_evict_first_policy();
+  uint8_t* const ring = rings + static_cast<size_t>(warp) * NS * Ring::kStageBytes;
+  const uint32_t bar0 = smem_u32(&full[warp][0]), ring_s = smem_u32(ring);
+  int in_slot = 0, slot = 0;
+  uint32_t parity = 0;
 
-  if (lane < NS) mbar_init(smem_u32(&full[warp][lane]), 1);
+  if (lane < NS) mbar_init(bar0 + lane * 8, 1);
   if (threadIdx.x == 0) abort_flag = 0;
   fence_mbar_init();
+  if (p.splits > 1) cluster_arrive_relaxed();  // waited for before anything is pushed
   pdl_wait();
   pdl_launch_dependents();
-  const int pos = p.pos[b];
-  if (pos < -1 || pos >= static_cast<long long>(p.max_pages) * p.page ||
-      (!p.sel && pos >= p.max_tiles * static_cast<long long>(kKv4Tile))) {
-    if (threadIdx.x == 0) record_error(kDevBadPosition);
-    return;  // the whole sequence and cluster, before any barrier: nothing is read or written
-  }
   __syncwarp();
 
-  // ---- this warp's tiles: index i -> stage i / ST -> tile
-  const int* row = p.table + static_cast<size_t>(b) * p.max_pages;
-  const int* sel = p.sel ? p.sel + (static_cast<size_t>(b) * p.hkv + kvh) * p.n_sel : nullptr;
-  const size_t head_bytes = static_cast<size_t>(tpp) * Ring::kTileBytes;
-  const int n_tiles = sel ? p.n_sel * tpp : pos / kKv4Tile + (pos >= 0);
-  const int groups = (n_tiles + ST - 1) / ST;  // stages of the whole sequence
-  const int g_lo = static_cast<int>(static_cast<long long>(groups) * split / p.n_splits);
-  const int g_hi = static_cast<int>(static_cast<long long>(groups) * (split + 1) / p.n_splits);
-  const int n_stages = max(0, (g_hi - g_lo - warp + W - 1) / W);
-  // lane's tile of the 32 that begin with tile index i0: its address, or its page's lookup
+  // ---- this CTA's tiles: its split of one pair, or its share of all
+  Kv4Run run;
+  Kv4RawQuery<D, W> raw;
+  int* const before = area;  // dealt: before[b] = weight of a kv head's pairs below sequence b
+  int u = 0, u1 = 0;         // dealt: the CTA's share, in weights of pairs: overhead, then tiles
+  if (p.splits) {
+    run.kvh = blockIdx.x / p.splits;
+    run.b = blockIdx.y;
+    kv4_load_query<D, W>(p, run.b, run.kvh, raw);
+    run.pos = p.pos[run.b];
+    bool bad;
+    run.n_tiles = kv4_seq_tiles(p, run.pos, bad);
+    if (bad) {
+      if (threadIdx.x == 0) record_error(kDevBadPosition);
+      if (p.splits > 1) cluster_wait_acquire();
+      return;  // the whole cluster: nothing is read or written
+    }
+    const int split = blockIdx.x % p.splits;
+    run.t_lo = static_cast<int>(static_cast<long long>(run.n_tiles) * split / p.splits);
+    run.t_hi = static_cast<int>(static_cast<long long>(run.n_tiles) * (split + 1) / p.splits);
+  } else {
+    int sum = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
+      const int i = b0 + threadIdx.x;
+      bool bad = false;
+      const int tiles = i < p.batch ? kv4_seq_tiles(p, p.pos[i], bad) : 0;
+      // a sequence without tiles: its rows become zeros, but for a bad position
+      if (i < p.batch && tiles == 0 && i % gridDim.x == blockIdx.x) {
+        if (bad) record_error(kDevBadPosition);
+        for (int h = 0; h < p.hkv; ++h) p.spans[static_cast<size_t>(i) * p.hkv + h] = make_int2(bad ? -1 : -2, 0);
+      }
+      const int mine = tiles ? tiles + Ring::kOverhead : 0;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int below = sum;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (w < warp) below += scan[w];
+        sum += scan[w];
+      }
+      if (i < p.batch) before[i] = below + incl - mine;
+      if (b0 + W * 32 < p.batch) __syncthreads();
+    }
+    if (threadIdx.x == 0) before[p.batch] = sum;
+    __syncthreads();
+    const int total = sum * p.hkv;  // below 2^30
+    const int n_cta = min(total, static_cast<int>(gridDim.x));
+    if (static_cast<int>(blockIdx.x) >= n_cta) return;
+    const int each = total / n_cta, rest = total - each * n_cta, me = blockIdx.x;
+    u = each * me + min(me, rest);
+    u1 = u + each + (me < rest);
+    int b = 0, hi = p.batch;  // the last sequence that begins at or below u, and has tiles
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (before[mid] * p.hkv <= u) b = mid;
+      else hi = mid;
+    }
+    run.b = b;
+    run.kvh = (u - before[b] * p.hkv) / (before[b + 1] - before[b]);
+  }
+  // dealt: the next pair of the share that has tiles in it; false behind the last.  A share may
+  // end inside a pair's overhead, which leaves it none of the tiles.
+  auto next = [&]() -> bool {
+    while (u < u1) {
+      const int weight = before[run.b + 1] - before[run.b];
+      const int in = u - before[run.b] * p.hkv - run.kvh * weight;
+      if (in >= weight) {  // on to the next pair
+        if (++run.kvh == p.hkv) {
+          run.kvh = 0;
+          do ++run.b;
+          while (before[run.b + 1] == before[run.b]);
+        }
+        continue;
+      }
+      const int out = min(weight, in + (u1 - u));
+      u += out - in;
+      run.n_tiles = weight - Ring::kOverhead;
+      run.t_lo = max(0, in - Ring::kOverhead);
+      run.t_hi = max(0, out - Ring::kOverhead);
+      if (run.t_hi > run.t_lo) return true;
+    }
+    return false;
+  };
+  // lane's tile of the 32 that begin with the warp's i0-th: its address, how much of it counts
   auto find = [&](int i0, int& left) -> const uint8_t* {
     const int i = i0 + lane;
     left = 0;
-    if (i >= n_stages * ST) return nullptr;
-    const int tile = (g_lo + warp + i / ST * W) * ST + i % ST;
-    if (tile >= n_tiles) return nullptr;
+    if (i >= run.n_stages << run.lg) return nullptr;
+    const int tile = run.t_lo + ((warp + (i >> run.lg) * W) << run.lg) + (i & ((1 << run.lg) - 1));
+    if (tile >= run.t_hi) return nullptr;
     int pg = tile / tpp;
     const int in_page = tile - pg * tpp;
-    if (sel) {  // an entry that does not rise above the one before it counts for nothing
-      const int at = pg;
-      pg = sel[at];
-      if (pg < 0 || pg >= p.max_pages || (at > 0 && pg <= sel[at - 1])) return nullptr;
+    if (p.sel) {  // an entry that does not rise above the one before it counts for nothing
+      const int* sel = p.sel + (static_cast<size_t>(run.b) * p.hkv + run.kvh) * p.n_sel + pg;
+      const int low = pg > 0 ? sel[-1] : -1;
+      pg = *sel;
+      if (pg < 0 || pg >= p.max_pages || pg <= low) return nullptr;
     }
     const long long first = static_cast<long long>(pg) * p.page + in_page * kKv4Tile;
-    if (first > pos) return nullptr;
-    const int id = row[pg];
+    if (first > run.pos) return nullptr;
+    const int id = p.table[static_cast<size_t>(run.b) * p.max_pages + pg];
     if (id < 0 || id >= p.n_pages) {
       record_error(kDevBadPosition);
       return nullptr;
     }
-    left = static_cast<int>(min(static_cast<long long>(kKv4Tile), pos + 1 - first));
-    return p.pool + (static_cast<size_t>(id) * p.hkv + kvh) * head_bytes + static_cast<size_t>(in_page) * Ring::kTileBytes;
+    left = static_cast<int>(min(static_cast<long long>(kKv4Tile), run.pos + 1 - first));
+    if (in_page && i & ((1 << run.lg) - 1)) left |= kBehind;
+    return p.pool + (static_cast<size_t>(id) * p.hkv + run.kvh) * head_bytes + static_cast<size_t>(in_page) * Ring::kTileBytes;
   };
-  uint8_t* ring = rings + static_cast<size_t>(warp) * NS * Ring::kStageBytes;
-  const uint64_t once = l2_evict_first_policy();
-  int left_now, left_next;
-  const uint8_t* at_now = find(0, left_now);
-  const uint8_t* at_next = n_stages * ST > 32 ? find(32, left_next) : nullptr;
-  // stage s into its slot: the lanes that hold its tiles copy them
-  auto issue = [&](int s) {
-    const int i = s * ST;
-    if (i > 0 && i % 32 == 0) {
-      at_now = at_next;
-      left_now = left_next;
-      if (i + 32 < n_stages * ST) at_next = find(i + 32, left_next);
-    }
-    const int mine = lane - i % 32;  // this lane's tile of the stage, if 0 .. ST - 1
-    const bool in = mine >= 0 && mine < ST;
-    const int count = __popc(__ballot_sync(0xffffffffu, in && left_now > 0));
-    const uint32_t bar = smem_u32(&full[warp][s % NS]);
-    if (in) left_s[warp][s % NS][mine] = left_now;
-    if (lane == 0) mbar_arrive_expect_tx(bar, count * Ring::kTileBytes);
+  // (kBehind: the tile lies behind the lane below's in memory and in its stage)
+  int left_now, left_next = 0;
+  const uint8_t *at_now, *at_next;
+  // the run's first lookups and query on their way (cluster: the query is already)
+  auto begin = [&]() {
+    run.lg = 0;
+    while ((2 << run.lg) <= ST && ((run.t_hi - run.t_lo) >> run.lg) > W) ++run.lg;
+    run.n_stages = max(0, (((run.t_hi - run.t_lo + (1 << run.lg) - 1) >> run.lg) - warp + W - 1) / W);
+    at_now = find(0, left_now);
+    at_next = run.n_stages << run.lg > 32 ? find(32, left_next) : nullptr;
+  };
+  if (!p.splits) {
+    if (!next()) return;
+    kv4_load_query<D, W>(p, run.b, run.kvh, raw);
+    run.pos = p.pos[run.b];
+  }
+  begin();
+
+  while (true) {
+    // ---- the run's first stages, then the query while they are on their way
+    int issued = 0;
+    unsigned whole = 0;  // bit s: every tile of the stage in slot s is there and full
+    auto issue = [&]() {  // the next stage into slot `in_slot`: the lanes that hold its tiles copy them
+      const int i = issued << run.lg;
+      if ((i & 31) == 0 && i > 0) {
+        at_now = at_next;
+        left_now = left_next;
+        if (i + 32 < run.n_stages << run.lg) at_next = find(i + 32, left_next);
+      }
+      const bool in = (lane >> run.lg) == ((i & 31) >> run.lg);
+      const int left = left_now & ~kBehind;
+      const unsigned some = __ballot_sync(0xffffffffu, in && left > 0);
+      const unsigned all = __ballot_sync(0xffffffffu, in && left == kKv4Tile);
+      // tiles that lie in a row are one copy, by the first one's lane
+      const unsigned first = __ballot_sync(0xffffffffu, in && left_now > 0 && !(left_now & kBehind));
+      const uint32_t bar = bar0 + in_slot * 8, mine = lane & ((1 << run.lg) - 1);
+      whole = (whole & ~(1u << in_slot)) | static_cast<unsigned>(__popc(all) == ST) << in_slot;
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(some) * Ring::kTileBytes);
+      __syncwarp();
+      if (in) {
+        left_s[warp][in_slot][mine] = left;
+        if (first >> lane & 1) {
+          // one and the lanes above that go on with it: none outside the stage, as `some` has none there
+          const int row = __ffs(static_cast<int>(~((some & ~first) >> lane >> 1)));
+          bulk_g2s(ring_s + in_slot * Ring::kStageBytes + mine * Ring::kTileBytes, at_now, row * Ring::kTileBytes, bar, once);
+        }
+      }
+      in_slot = in_slot + 1 == NS ? 0 : in_slot + 1;
+      ++issued;
+    };
+    // a stage with fewer tiles than it has room for: the others count for nothing
+    if (lane < ST * NS) left_s[warp][lane / ST][lane % ST] = 0;
     __syncwarp();
-    if (in && left_now > 0)
-      bulk_g2s(smem_u32(ring + (s % NS) * Ring::kStageBytes + mine * Ring::kTileBytes), at_now, Ring::kTileBytes, bar, once);
-  };
-  int issued = 0;
-  for (; issued < min(NS, n_stages); ++issued) issue(issued);
-
-  // ---- the query, while the first stages are on their way
-  kv4_load_query<D, W * 32>(p, rope, b, kvh, max(pos, 0), Q);
-  uint32_t qb[G][4][2];
-  float qs[G][2], unit[2] = {Q.unit[2 * c], Q.unit[2 * c + 1]};
-  Kv4State<D> st;
+    while (issued < min(NS, run.n_stages)) issue();
+    kv4_prepare_query<D, W>(p, rope, max(run.pos, 0), raw, Q);
+    __syncthreads();
+    uint32_t qb[G][4][2];
+    float qs[G][2], unit[2] = {Q.unit[2 * c], Q.unit[2 * c + 1]};
+    Kv4State<D> st;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
+    for (int g = 0; g < G; ++g) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      qb[g][k][0] = Q.b[g][k][0][lane];
-      qb[g][k][1] = Q.b[g][k][1][lane];
+      for (int k = 0; k < 4; ++k) {
+        qb[g][k][0] = *reinterpret_cast<const uint32_t*>(&Q.b[g][k][0][lane][0]);
+        qb[g][k][1] = *reinterpret_cast<const uint32_t*>(&Q.b[g][k][1][lane][0]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qs[g][e] = Q.sum[g][2 * c + e];
+        st.m[g][e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st.o[g][i][0] = st.o[g][i][1] = st.o[g][i][2] = st.o[g][i][3] = 0.f;
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      qs[g][e] = Q.sum[g][2 * c + e];
-      st.m[g][e] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) st.o[g][i][0] = st.o[g][i][1] = st.o[g][i][2] = st.o[g][i][3] = 0.f;
-  }
-  st.l[0] = st.l[1] = 0.f;
-  st.r[0] = st.r[1] = -1e30f;
+    st.l[0] = st.l[1] = 0.f;
+    st.r[0] = st.r[1] = -1e30f;
 
-  int s = 0;
-  for (; s < n_stages; ++s) {
-    // a wait that runs out ends this warp's work: the result is void, and reported
-    const bool here = mbar_wait_bounded(smem_u32(&full[warp][s % NS]), (s / NS) & 1, &abort_flag, kDevTimeoutFull);
-    if (!__all_sync(0xffffffffu, here)) break;
-    int left[ST];
+    int done = 0;
+    for (; done < run.n_stages; ++done) {
+      const uint32_t bar = bar0 + slot * 8;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        // a wait that runs out ends this warp's work: the result is void, and reported
+        const bool here = mbar_wait_bounded(bar, parity, &abort_flag, kDevTimeoutFull);
+        if (!__all_sync(0xffffffffu, here)) break;
+      }
+      const uint8_t* stage = ring + slot * Ring::kStageBytes;
+      if (whole >> slot & 1) {
 #pragma unroll
-    for (int n = 0; n < ST; ++n) left[n] = left_s[warp][s % NS][n];
-    kv4_tiles<D, ST>(ring + (s % NS) * Ring::kStageBytes, Ring::kTileBytes, left, qb, qs, unit, st);
-    __syncwarp();  // every lane has read the slot
-    if (issued < n_stages) issue(issued++);
-  }
-  if (s < n_stages)  // copies still in flight land before the ring is used for anything else
-    for (; s < issued; ++s) {
+        for (int n = 0; n < ST; n += NT)
+          kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, nullptr, qb, qs, unit, st);
+      } else {
+#pragma unroll 1
+        for (int n = 0; n < 1 << run.lg; n += NT)
+          kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, &left_s[warp][slot][n], qb, qs, unit, st);
+      }
+      __syncwarp();  // every lane has read the slot
+      if (issued < run.n_stages) issue();
+      if (++slot == NS) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+    for (; done < issued; ++done) {  // given up: copies in flight land before the ring is used otherwise
       const uint64_t t0 = globaltimer();
-      while (!mbar_try_wait(smem_u32(&full[warp][s % NS]), (s / NS) & 1))
+      while (!mbar_try_wait(bar0 + slot * 8, parity))
         if (globaltimer() - t0 > B2_WAIT_TIMEOUT_NS) {
           record_error(kDevTimeoutDrain);
           break;
         }
+      if (++slot == NS) {
+        slot = 0;
+        parity ^= 1;
+      }
     }
 
-  // ---- the warp's sums over its token lanes, then the warps through shared memory
-  float(*mo)[kKv4MaxGroup][D + 1] = reinterpret_cast<float(*)[kKv4MaxGroup][D + 1]>(rings);
-  static_assert(W * kKv4MaxGroup * (D + 1) * 4 <= kv4_decode_smem<D, W>(), "the sums fit the rings");
-  __syncthreads();  // every warp is done with its ring
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-#pragma unroll
-    for (int o = 4; o <= 16; o <<= 1) {
-      st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], o);
-#pragma unroll
-      for (int g = 0; g < G; ++g) st.m[g][e] += __shfl_xor_sync(0xffffffffu, st.m[g][e], o);
+    // ---- the next run's lookups set out before this one's sums are joined
+    const int b = run.b, kvh = run.kvh, t_lo = run.t_lo, t_hi = run.t_hi, n_tiles = run.n_tiles;
+    const bool more = !p.splits && next();
+    if (more) {
+      kv4_load_query<D, W>(p, run.b, run.kvh, raw);
+      if (run.b != b) run.pos = p.pos[run.b];
+      begin();
     }
-    if (gl == 0) {
-      ml[warp][2 * c + e] = st.l[e];
-      mr[warp][2 * c + e] = st.r[e];
-    }
-  }
+
+    // ---- the warp's sums over its token lanes, then the warps through shared memory
+    float(*mo)[kKv4MaxGroup][D + 1] = reinterpret_cast<float(*)[kKv4MaxGroup][D + 1]>(rings);
+    static_assert(W * kKv4MaxGroup * (D + 1) * 4 <= kv4_decode_smem<D, W>(), "the sums fit the rings");
+    __syncthreads();  // every warp is done with its ring
 #pragma unroll
-  for (int g = 0; g < G; ++g)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float scale = i & 1 ? 1048576.f : 16777216.f;  // 2^20, 2^24
+      for (int o = 4; o <= 16; o <<= 1) {
+        st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], o);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mo[warp][2 * c + e][64 * g + 8 * gl + i] = fmaf(st.o[g][i][e], scale, st.m[g][e]);
-        mo[warp][2 * c + e][64 * g + 8 * gl + 4 + i] = fmaf(st.o[g][i][2 + e], scale, st.m[g][e]);
+        for (int g = 0; g < G; ++g) st.m[g][e] += __shfl_xor_sync(0xffffffffu, st.m[g][e], o);
+      }
+      if (gl == 0) {
+        ml[warp][2 * c + e] = st.l[e];
+        mr[warp][2 * c + e] = st.r[e];
       }
     }
-  __syncthreads();
-  // the CTA's sums over Q's memory (last read before the loop): o [grp][D], then R and L
-  float* cta = reinterpret_cast<float*>(&Q);
-  static_assert(sizeof(Kv4Query<D>) >= kKv4MaxGroup * (D + 2) * 4, "the CTA's sums fit the query's memory");
-  for (int e = threadIdx.x; e < grp * D; e += W * 32) {
-    const int j = e / D, d = e % D;
-    float R = -1e30f, L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      if (ml[w][j] != 0.f) R = fmaxf(R, mr[w][j]);
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (ml[w][j] == 0.f) continue;
-      const float f = kv4_ex2(mr[w][j] - R);
-      L = fmaf(ml[w][j], f, L);
-      O = fmaf(mo[w][j][d], f, O);
-    }
-    if (p.n_splits == 1) {
-      kv4_store_out(p, b, kvh * grp + j, D, d, L == 0.f ? 0.f : O / L);
-    } else {
-      float* part = p.clustered ? cta : p.part + ((static_cast<size_t>(b) * p.hkv + kvh) * p.n_splits + split) * grp * (D + 2);
-      part[e] = O;
-      if (d == 0) {
-        part[grp * D + j] = R;
-        part[grp * D + grp + j] = L;
+      for (int i = 0; i < 4; ++i) {
+        const float scale = i & 1 ? 1048576.f : 16777216.f;  // 2^20, 2^24
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float sum = i & 1 ? st.o[g][i][e] - st.o[g][i - 1][e] : st.o[g][i][e];
+          mo[warp][2 * c + (e & 1)][64 * g + 8 * gl + 2 * (e & 2) + i] = fmaf(sum, scale, st.m[g][e & 1]);
+        }
+      }
+    if (p.splits > 1) cluster_wait_acquire();  // the cluster's CTAs have all begun
+    __syncthreads();
+    const bool alone = p.splits ? p.splits == 1 : t_hi - t_lo == n_tiles;
+    const int split = p.splits ? blockIdx.x % p.splits : 0;
+    const int share = p.splits ? (grp * D + p.splits - 1) / p.splits : 1;  // outputs that a CTA of the cluster joins
+    const uint32_t push_o = smem_u32(area), push_rl = push_o + kPush * 4;
+    float* part = p.part + (2 * static_cast<size_t>(blockIdx.x) + (t_lo == 0)) * kv4_part_floats(grp, D);
+    for (int e = threadIdx.x; e < grp * D; e += W * 32) {
+      const int j = e / D, d = e % D;
+      float R = -1e30f, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (ml[w][j] != 0.f) R = fmaxf(R, mr[w][j]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (ml[w][j] == 0.f) continue;
+        const float f = kv4_ex2(mr[w][j] - R);
+        L = fmaf(ml[w][j], f, L);
+        O = fmaf(mo[w][j][d], f, O);
+      }
+      if (alone) {
+        kv4_store_out(p, b, kvh * grp + j, D, d, L == 0.f ? 0.f : O / L);
+      } else if (p.splits) {
+        st_dsmem_f32(push_o + (split * share + e % share) * 4, e / share, O);
+        if (d == 0)
+          for (int k = 0; k < p.splits; ++k) {
+            st_dsmem_f32(push_rl + ((split * kKv4MaxGroup + j) * 2) * 4, k, R);
+            st_dsmem_f32(push_rl + ((split * kKv4MaxGroup + j) * 2 + 1) * 4, k, L);
+          }
+      } else {
+        part[e] = O;
+        if (d == 0) {
+          part[grp * D + j] = R;
+          part[grp * D + grp + j] = L;
+        }
       }
     }
-  }
-  if (!p.clustered) return;
-  cluster_sync_all();
-  // every CTA of the cluster joins a share of the outputs
-  const uint32_t base = smem_u32(cta);
-  for (int e = split * W * 32 + threadIdx.x; e < grp * D; e += p.n_splits * W * 32) {
-    const int j = e / D;
-    float R = -1e30f, L = 0.f, O = 0.f;
-    for (int k = 0; k < p.n_splits; ++k)
-      if (ld_dsmem_f32(base + (grp * D + grp + j) * 4, k) != 0.f) R = fmaxf(R, ld_dsmem_f32(base + (grp * D + j) * 4, k));
-    for (int k = 0; k < p.n_splits; ++k) {
-      const float l = ld_dsmem_f32(base + (grp * D + grp + j) * 4, k);
-      const float f = l == 0.f ? 0.f : kv4_ex2(ld_dsmem_f32(base + (grp * D + j) * 4, k) - R);
-      const float o = ld_dsmem_f32(base + e * 4, k);
-      if (l != 0.f) {
-        L = fmaf(l, f, L);
-        O = fmaf(o, f, O);
+    if (p.splits) {
+      if (alone) return;
+      // ---- the cluster: this CTA's share of the outputs from what all have pushed
+      cluster_sync_all();
+      const float* o = reinterpret_cast<const float*>(area);
+      const float* rl = o + kPush;
+      for (int i = threadIdx.x; i < share; i += W * 32) {
+        const int e = split * share + i, j = e / D;
+        if (e >= grp * D) break;
+        float R = -1e30f, L = 0.f, O = 0.f;
+        for (int k = 0; k < p.splits; ++k)
+          if (rl[(k * kKv4MaxGroup + j) * 2 + 1] != 0.f) R = fmaxf(R, rl[(k * kKv4MaxGroup + j) * 2]);
+        for (int k = 0; k < p.splits; ++k) {
+          const float l = rl[(k * kKv4MaxGroup + j) * 2 + 1];
+          if (l == 0.f) continue;
+          const float f = kv4_ex2(rl[(k * kKv4MaxGroup + j) * 2] - R);
+          L = fmaf(l, f, L);
+          O = fmaf(o[k * share + i], f, O);
+        }
+        kv4_store_out(p, b, kvh * grp + j, D, e % D, L == 0.f ? 0.f : O / L);
       }
+      return;
     }
-    kv4_store_out(p, b, kvh * grp + j, D, e % D, L == 0.f ? 0.f : O / L);
+    if (threadIdx.x == 0) {
+      int2* span = p.spans + static_cast<size_t>(b) * p.hkv + kvh;
+      if (t_lo == 0) span->x = alone ? -1 : blockIdx.x;
+      if (t_hi == n_tiles) span->y = blockIdx.x;
+    }
+    if (!more) return;
+    fence_proxy_async();  // the rings' bytes go from these threads back to the copies
+    __syncthreads();      // the sums in the rings have been read
   }
-  cluster_sync_all();  // no CTA's shared memory goes while another reads it
 }
 
-// Joins the splits: one CTA per (q head, sequence), a thread per dim.
+// Joins the pairs that several CTAs share, and clears the rows of sequences without tokens:
+// grid (kv head, sequence, share of the heads).  A thread joins D / 64 outputs of one head (at 40
+// heads of 64 one each measured 2.3 us less than four, at 8 of 256 four 3 us less than one);
+// threads beyond the outputs take every further part of them (few pairs, many parts each).
+// The parts' loads set out together: the kernel is two trips to L2 long.
+constexpr int kKv4JoinMost = 512;
 template <int D>
-__global__ void __launch_bounds__(D) kv4_combine_kernel(const Kv4DecodeParams p) {
-  const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x, grp = p.hq / p.hkv;
+__global__ void __launch_bounds__(kKv4JoinMost) kv4_join_kernel(const Kv4DecodeParams p) {
+  constexpr int V = D / 64;
+  __shared__ float sh[2 + V][kKv4JoinMost];
+  const int kvh = blockIdx.x, b = blockIdx.y, grp = p.hq / p.hkv, tid = threadIdx.x;
+  const int heads = grp / gridDim.z, j0 = blockIdx.z * heads, quads = heads * D / V;
   pdl_wait();
   pdl_launch_dependents();
-  const int pos = p.pos[b];
-  if (pos < -1 || pos >= static_cast<long long>(p.max_pages) * p.page ||
-      (!p.sel && pos >= p.max_tiles * static_cast<long long>(kKv4Tile)))
-    return;
-  const int j = head % grp;
-  const size_t step = static_cast<size_t>(grp) * (D + 2);
-  const float* part = p.part + (static_cast<size_t>(b) * p.hkv + head / grp) * p.n_splits * step;
-  float R = -1e30f, L = 0.f, O = 0.f;
-  for (int s = 0; s < p.n_splits; ++s)
-    if (part[s * step + grp * D + grp + j] != 0.f) R = fmaxf(R, part[s * step + grp * D + j]);
-  for (int s = 0; s < p.n_splits; ++s) {
-    const float l = part[s * step + grp * D + grp + j];
-    if (l == 0.f) continue;
-    const float w = kv4_ex2(part[s * step + grp * D + j] - R);
-    L = fmaf(l, w, L);
-    O = fmaf(part[s * step + j * D + d], w, O);
+  const int2 span = p.spans[static_cast<size_t>(b) * p.hkv + kvh];
+  if (span.x == -1) return;
+  const int step = kv4_part_floats(grp, D), n = span.x < 0 ? 0 : span.y - span.x + 1;
+  const int slices = blockDim.x / quads;  // 1 where the heads have more outputs than this is 4 of
+  const int e = (tid % quads) * V, slice = tid / quads;
+  const int at = j0 * D + e, rl = grp * D + j0 + e / D;
+  const float* base = p.part + (2 * static_cast<size_t>(max(span.x, 0)) + 1) * step;  // the pair's first part
+  float R = -1e30f, L = 0.f, O[V] = {};
+  auto add = [&](float r, float l, const float (&o)[V]) {
+    if (l == 0.f) return;
+    const float m = fmaxf(R, r), f = kv4_ex2(R - m), g = kv4_ex2(r - m);
+    R = m;
+    L = fmaf(L, f, l * g);
+#pragma unroll
+    for (int i = 0; i < V; ++i) O[i] = fmaf(O[i], f, o[i] * g);
+  };
+  for (int k0 = slice; k0 < n; k0 += 4 * slices) {
+    float r[4], l[4], o[4][V];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // part k > 0 is the first place of the k-th CTA behind the span's first
+      const int k = k0 + i * slices;
+      const float* part = base + (k ? static_cast<ptrdiff_t>(2 * k - 1) * step : 0);
+      r[i] = k < n ? part[rl] : 0.f;
+      l[i] = k < n ? part[rl + grp] : 0.f;
+#pragma unroll
+      for (int x = 0; x < V; ++x) o[i][x] = k < n ? part[at + x] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(r[i], l[i], o[i]);
   }
-  kv4_store_out(p, b, head, D, d, L == 0.f ? 0.f : O / L);
+  if (slices > 1) {
+    sh[0][tid] = R;
+    sh[1][tid] = L;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sh[2 + i][tid] = O[i];
+    __syncthreads();
+    if (slice > 0) return;
+    for (int k = 1; k < slices; ++k) {
+      const int t = tid + k * quads;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = sh[2 + i][t];
+      add(sh[0][t], sh[1][t], o);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    kv4_store_out(p, b, kvh * grp + j0 + e / D, D, e % D + i, L == 0.f ? 0.f : O[i] / L);
 }
 
 }  // namespace b2

@@ -83,24 +83,29 @@ auto kv4_by_dim(int head_dim, F f) {
                            : f(std::integral_constant<int, 256>());
 }
 
+constexpr int kKv4DecodeWarps = 4;
+
 struct Kv4DecodePlan {
-  int tiles, warps, n_splits, clustered;
-  size_t ws_bytes;
+  int tiles, splits, ctas;  // splits 0: tiles dealt over ctas
+  size_t span_bytes, ws_bytes;
 };
 
-// Splits until the CTAs are about four per SM, no warp below two tiles; up to 16 are joined
-// in a cluster.
+// A cluster per (sequence, kv head) while that leaves no warp more than four tiles and the
+// clusters fit the GPU at once; else the tiles are dealt over as many CTAs as it holds, each
+// with two per warp at least.
 Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int tokens, int sms) {
-  Kv4DecodePlan pl;
+  Kv4DecodePlan pl = {};
+  constexpr int W = kKv4DecodeWarps;
   pl.tiles = (tokens + 15) / 16;
-  pl.warps = 4;
-  const long long pairs = static_cast<long long>(batch) * hkv;
-  const long long most = std::max(1, pl.tiles / (2 * pl.warps));
-  long long s = std::max(1LL, std::min(most, (4LL * sms + pairs - 1) / pairs));
-  if (s > 16 && 16 * pairs >= sms) s = 16;
-  pl.n_splits = static_cast<int>(s);
-  pl.clustered = s > 1 && s <= 16;
-  pl.ws_bytes = s > 16 ? static_cast<size_t>(batch) * hq * pl.n_splits * (head_dim + 2) * sizeof(float) : 0;
+  const long long pairs = static_cast<long long>(batch) * hkv, slots = (head_dim == 256 ? 2LL : 4LL) * sms;
+  const int s = std::min(16, (pl.tiles + W - 1) / W);
+  if (pairs * s <= slots && pl.tiles <= 4 * W * s) {
+    pl.splits = s;
+    return pl;
+  }
+  pl.ctas = static_cast<int>(std::min(slots, (pairs * pl.tiles + 2 * W - 1) / (2 * W)));
+  pl.span_bytes = (static_cast<size_t>(pairs) * 8 + 15) / 16 * 16;
+  pl.ws_bytes = pl.span_bytes + static_cast<size_t>(pl.ctas) * 2 * b2::kv4_part_floats(hq / hkv, head_dim) * sizeof(float);
   return pl;
 }
 
@@ -228,6 +233,7 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
       kv4_decode_plan(batch, n_q_heads, n_kv_heads, head_dim, kv4_decode_tokens(n_sel, page, max_len), di.sms);
   if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)))
     return fail(B2_ERR_WORKSPACE, "kv4 decode needs %zu bytes of 16-byte aligned workspace", pl.ws_bytes);
+  if ((pl.tiles + 16LL) * n_kv_heads > (1LL << 30)) return fail(B2_ERR_ARG, "a sequence of over 2^34 tokens x kv heads");
   b2::Kv4DecodeParams p = {};
   p.q = q;
   p.ld_q = ld_q;
@@ -236,7 +242,6 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
   p.pos = pos;
   p.sel = sel;
   p.out = out;
-  p.part = static_cast<float*>(workspace);
   p.ldo = ldo;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.batch = batch;
@@ -246,15 +251,14 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
   p.max_pages = max_pages;
   p.n_pages = n_pages;
   p.n_sel = n_sel;
-  p.n_splits = pl.n_splits;
-  p.clustered = pl.clustered;
+  p.splits = pl.splits;
   p.max_tiles = pl.tiles;
   p.out_f32 = (flags & B2_KV4_OUT_F32) ? 1 : 0;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
   cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    auto kernel = b2::kv4_decode_kernel<D, 4>;
-    constexpr size_t smem = b2::kv4_decode_smem<D, 4>();
+    auto kernel = b2::kv4_decode_kernel<D, kKv4DecodeWarps>;
+    constexpr size_t smem = b2::kv4_decode_smem<D, kKv4DecodeWarps>();
     static std::atomic<unsigned long long> ready{0};  // devices on which the kernel's attributes are set
     int dev = 0;
     cudaGetDevice(&dev);
@@ -264,18 +268,36 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
       if (r != cudaSuccess) return r;
       ready.fetch_or(1ull << dev);
     }
-    Kv4Launch l(dim3(pl.n_splits, n_kv_heads, batch), pl.warps * 32, stream, smem);
-    if (pl.clustered) l.cluster(pl.n_splits);
-    return cudaLaunchKernelEx(&l.cfg, kernel, p, rope);
+    if (pl.splits) {
+      Kv4Launch l(dim3(pl.splits * n_kv_heads, batch, 1), kKv4DecodeWarps * 32, stream, smem);
+      l.cluster(pl.splits);
+      return cudaLaunchKernelEx(&l.cfg, kernel, p, rope);
+    }
+    // dealt over the grid, a slice of the batch at a time: the weights of a slice fit 32 bits
+    const int slice = static_cast<int>(std::min<long long>(b2::kKv4MaxDealt, (1LL << 30) / ((pl.tiles + 16LL) * n_kv_heads)));
+    for (int b0 = 0; b0 < batch; b0 += slice) {
+      b2::Kv4DecodeParams part = p;
+      part.batch = std::min(slice, batch - b0);
+      part.q = q + b0 * ld_q;
+      part.table = table + static_cast<size_t>(b0) * max_pages;
+      part.pos = pos + b0;
+      if (sel) part.sel = sel + static_cast<size_t>(b0) * n_kv_heads * n_sel;
+      part.out = static_cast<char*>(out) + b0 * ldo * (p.out_f32 ? 4 : 2);
+      part.spans = static_cast<int2*>(workspace);
+      part.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.span_bytes);
+      Kv4Launch l(dim3(pl.ctas, 1, 1), kKv4DecodeWarps * 32, stream, smem);
+      cudaError_t r = cudaLaunchKernelEx(&l.cfg, kernel, part, rope);
+      if (r != cudaSuccess) return r;
+      // few pairs, of which one may have a hundred parts: a CTA per head, four threads per output
+      const int grp = n_q_heads / n_kv_heads;
+      const bool few = part.batch * n_kv_heads < di.sms;
+      Kv4Launch j(dim3(n_kv_heads, part.batch, few ? grp : 1), few ? 256 : grp * 64, stream);
+      r = cudaLaunchKernelEx(&j.cfg, b2::kv4_join_kernel<D>, part);
+      if (r != cudaSuccess) return r;
+    }
+    return cudaSuccess;
   });
   if (e != cudaSuccess) return cuda_fail(e, "kv4 decode launch");
-  if (pl.ws_bytes) {
-    Kv4Launch c(dim3(n_q_heads, batch, 1), head_dim, stream);
-    e = kv4_by_dim(head_dim, [&](auto d) {
-      return cudaLaunchKernelEx(&c.cfg, b2::kv4_combine_kernel<decltype(d)::value>, p);
-    });
-    if (e != cudaSuccess) return cuda_fail(e, "kv4 combine launch");
-  }
   return B2_OK;
 }
 

@@ -45,29 +45,6 @@ __global__ void __launch_bounds__(kKv4CopyThreads) kv4_copy_kernel(const Kv4Page
   kv4_copy_page(d, blockIdx.y, s, t, blockIdx.x, gridDim.x);
 }
 
-// Sum of v over the threads below this one; total = over all (blockDim.x threads, 32 warps at most).
-__device__ __forceinline__ int kv4_block_before(int v, int* warps, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  int s = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += x;
-  }
-  __syncthreads();  // the array's last use is over
-  if (lane == 31) warps[warp] = s;
-  __syncthreads();
-  int x = lane < nw ? warps[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  total = __shfl_sync(0xffffffffu, x, 31);
-  const int before = __shfl_sync(0xffffffffu, x, max(warp - 1, 0));
-  return s - v + (warp ? before : 0);
-}
-
 struct Kv4ReorderParams {
   Kv4PageData data;
   const int *table, *lens, *refs, *parent, *reserve;  // reserve may be null
