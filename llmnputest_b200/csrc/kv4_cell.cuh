@@ -37,6 +37,14 @@ struct Kv4Rope {
   int on;
 };
 
+// A kernel parameter's table entry by a lane's own index: through its generic address, as the
+// constant port would take the 32 lanes' indices one by one.
+__device__ __forceinline__ double kv4_turn(const Kv4Rope& rope, int i) {
+  double t;
+  asm("ld.f64 %0, [%1];" : "=d"(t) : "l"(rope.turn + i));
+  return t;
+}
+
 // byte of K code word w (8 dims) of token t: dims 8 w .. 8 w + 7 of the cell's 64
 __host__ __device__ constexpr int kv4_k_word(int t, int w) {
   return (t % 8) * 64 + (w / 2) * 16 + (t / 8) * 8 + (w % 2) * 4;

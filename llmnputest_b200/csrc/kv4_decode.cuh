@@ -88,14 +88,6 @@ __device__ __forceinline__ void kv4_load_query(const Kv4DecodeParams& p, int b, 
   }
 }
 
-// A kernel parameter's table entry by a lane's own index: through its generic address, as the
-// constant port would take the 32 lanes' indices one by one.
-__device__ __forceinline__ double kv4_turn(const Kv4Rope& rope, int i) {
-  double t;
-  asm("ld.f64 %0, [%1];" : "=d"(t) : "l"(rope.turn + i));
-  return t;
-}
-
 template <int D, int W>
 __device__ __forceinline__ void kv4_prepare_query(const Kv4DecodeParams& p, const Kv4Rope& rope, int pos,
                                                   Kv4RawQuery<D, W>& q, Kv4Query<D>& Q) {
