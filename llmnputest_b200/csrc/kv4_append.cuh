@@ -14,9 +14,11 @@
 // error; the few that lie within the bound of a border (1 in 10^4 or less) are made again in
 // fp64.
 //
-// One CTA per (page of a sequence, kv head), a warp per token, lanes over the dims; the page's
-// summary needs no second pass that way.  Codes go through shared memory into the cell's
-// words.  Bound by instruction issue (about 115 a token and head of 64 dims).
+// One CTA per (page of a sequence, kv head), so that the page's summary needs no second pass.
+// D / 8 lanes have a token, each two quads of dims (4 l and D / 2 + 4 l: the pairs that turn
+// together), so that what is done once per 64 values is done for 32 / (D / 8) tokens at a
+// time; a warp per token measured 282 instructions a token and head of 64 dims and 26 us for
+// 8192 tokens of 8 heads.  The codes are put together in shared memory as the cell's bytes.
 #pragma once
 
 #include "kv4_cell.cuh"
@@ -36,74 +38,167 @@ struct Kv4RowsParams {
   __nv_bfloat16* summary;  // [n_pages][hkv][2][D] min, max of the page's keys, or null
   int rows, batch, hkv, page, max_pages, n_pages;
   int is_f32;  // k and v are fp32 (else bf16)
+  int wide;    // append: four values of a row can be loaded at once
 };
 
-// The least and the largest of a warp's values (sm_100a reduces them in one instruction).
-__device__ __forceinline__ float warp_redux_min(float v) {
-  float r;
-  asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float warp_redux_max(float v) {
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
-// The codes of a warp's 64 values (lane: x0, x1; f0, f1 their fp32 roundings): d and m, by lane
-// the two codes.  T is double where the values are not fp32 themselves.
-template <typename T>
-__device__ __forceinline__ void kv4_quantise(T x0, T x1, float f0, float f1, uint32_t& c0, uint32_t& c1,
-                                             uint32_t& meta) {
-  const float mn = warp_redux_min(fminf(f0, f1)), mx = warp_redux_max(fmaxf(f0, f1));
-  // a value that is not finite makes its 64 NaN: 4 bits have no such value
-  if (__any_sync(0xffffffffu, !(fabsf(f0) < INFINITY) || !(fabsf(f1) < INFINITY))) {
-    c0 = c1 = 0;
-    meta = 0x7FC00000u | (__float_as_uint(kKv4MinStep) >> 16);
-    return;
-  }
-  const float m = round_bf16(mn);  // the rounding is monotone: that of the least x itself
-  // (max x - m) / 15: f32 is off by 2^-22 of it, or of max x, at most; where bf16's rounding
-  // could see that, in fp64
-  float q = (mx - m) * (1.f / 15.f);
-  const float slack = (fabsf(mx) + fabsf(m)) * 2.4e-7f;
-  if (round_bf16(q - slack) != round_bf16(q + slack)) {
-    double top = fmax(static_cast<double>(x0), static_cast<double>(x1));
+// The choices that fp32 cannot make, out of line: a few in 10^4.
+template <int RL>
+__device__ __noinline__ float kv4_step_fp64(double top, float m) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    q = static_cast<float>((top - m) / 15.0);
-  }
-  const float d = fmaxf(round_bf16(q), kKv4MinStep), inv = __frcp_rn(d);
-  // (x - m) / d + 1/2 is off by `tol` at most: 2^-21 of what enters it
-  const float tol = fmaf((fmaxf(fabsf(mx), fabsf(mn)) + fabsf(m)) * inv, 4.8e-7f, 1e-5f);
-  auto code = [&](T x, float f) -> uint32_t {
-    const float y = fmaf(f - m, inv, 0.5f);
-    const float lo = fminf(fmaxf(floorf(y - tol), 0.f), 15.f), hi = fminf(fmaxf(floorf(y + tol), 0.f), 15.f);
-    if (lo == hi) return static_cast<uint32_t>(lo);
-    return static_cast<uint32_t>(fmin(fmax(floor((static_cast<double>(x) - m) / d + 0.5), 0.0), 15.0));
-  };
-  c0 = code(x0, f0);
-  c1 = code(x1, f1);
-  meta = (__float_as_uint(d) >> 16) | (__float_as_uint(m) & 0xFFFF0000u);
+  for (int o = RL / 2; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return static_cast<float>((top - m) / 15.0);
+}
+__device__ __noinline__ uint32_t kv4_code_fp64(double x, float m, float d) {
+  return static_cast<uint32_t>(fmin(fmax(floor((x - m) / d + 0.5), 0.0), 15.0));
 }
 
-// Four codes in four bytes as 16 bits of nibbles.
-__device__ __forceinline__ uint32_t kv4_nibbles(uint32_t bytes) {
-  const uint32_t y = (bytes | bytes >> 4) & 0x00FF00FFu;
-  return (y | y >> 8) & 0xFFFFu;
+// cos and sin of u turns in fp64: to the nearest quarter turn, then the Taylor series of an
+// angle of pi/4 at most (the first term left out is below 3e-18).  Without branches, so that
+// several angles are evaluated side by side: a library sincospi each measured 0.7 us an angle.
+__device__ __forceinline__ void kv4_cos_sin(double u, double& cs, double& sn) {
+  const double quarter = rint(4.0 * u);
+  const double x = fma(quarter, -0.25, u) * 6.283185307179586476925287, y = x * x;
+  double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;  // 1 / 17!, 1 / 16!
+  s = fma(s, y, -1.0 / 1307674368000.0);
+  c = fma(c, y, -1.0 / 87178291200.0);
+  s = fma(s, y, 1.0 / 6227020800.0);
+  c = fma(c, y, 1.0 / 479001600.0);
+  s = fma(s, y, -1.0 / 39916800.0);
+  c = fma(c, y, -1.0 / 3628800.0);
+  s = fma(s, y, 1.0 / 362880.0);
+  c = fma(c, y, 1.0 / 40320.0);
+  s = fma(s, y, -1.0 / 5040.0);
+  c = fma(c, y, -1.0 / 720.0);
+  s = fma(s, y, 1.0 / 120.0);
+  c = fma(c, y, 1.0 / 24.0);
+  s = fma(s, y, -1.0 / 6.0);
+  c = fma(c, y, -0.5);
+  s = fma(s * y, x, x);
+  c = fma(c, y, 1.0);
+  const int k = static_cast<int>(static_cast<long long>(quarter)) & 3;
+  cs = k & 1 ? s : c;
+  sn = k & 1 ? c : s;
+  if (k == 1 || k == 2) cs = -cs;
+  if (k >= 2) sn = -sn;
+}
+
+// Two fp32 as bf16, hi in the upper half.
+__device__ __forceinline__ uint32_t bf16x2_of(float hi, float lo) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// The codes of 64 values, NV in each of RL lanes in a row (x(i) in fp64; f their fp32
+// roundings), 4 bits each from the lowest, and (d, m).  The whole warp takes part.
+template <int RL, int NV, typename X>
+__device__ __forceinline__ uint32_t kv4_quantise(const X& x, const float (&f)[NV], uint32_t& meta) {
+  float mn = f[0], mx = f[0], odd = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    mn = fminf(mn, f[i]);
+    mx = fmaxf(mx, f[i]);
+    odd = fmaf(f[i], 0.f, odd);  // NaN if a value is not finite
+  }
+#pragma unroll
+  for (int o = RL / 2; o > 0; o >>= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  const unsigned bad = __ballot_sync(0xffffffffu, isnan(odd));
+  const uint32_t mb = bf16x2_of(mn, mn) & 0xFFFF0000u;  // the rounding is monotone: that of the least x itself
+  const float m = __uint_as_float(mb);
+  // (max x - m) / 15: fp32 is off by 2^-22 of it, or of max x, at most; where bf16's rounding
+  // could see that, in fp64
+  const float q = (mx - m) * (1.f / 15.f);
+  const float reach = fmaxf(fabsf(mx), fabsf(mn)) + fabsf(m), slack = reach * 2.4e-7f;
+  const uint32_t both = bf16x2_of(q + slack, q - slack);
+  float d = __uint_as_float(both & 0xFFFF0000u);
+  const bool unsure = both >> 16 != (both & 0xFFFFu);
+  if (__any_sync(0xffffffffu, unsure)) {
+    double top = x(0);
+#pragma unroll
+    for (int i = 1; i < NV; ++i) top = fmax(top, x(i));
+    const float sure = round_bf16(kv4_step_fp64<RL>(top, m));
+    if (unsure) d = sure;
+  }
+  d = fmaxf(d, kKv4MinStep);
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(d));
+  // (x - m) / d, off by 2^-21 of what enters it at most, to the nearest whole number in the low
+  // bits of 3 * 2^22 + it; nearer than that to half a step between two, in fp64
+  const float near = 0.5f - fmaf(reach * inv, 4.8e-7f, 1e-5f), nm = -m * inv;
+  uint32_t code = 0;
+  float off = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const float z = fminf(fmaxf(fmaf(f[i], inv, nm), 0.f), 15.f), r = z + 12582912.f;
+    off = fmaxf(off, fabsf(z - (r - 12582912.f)));
+    code |= (__float_as_uint(r) & 15u) << (4 * i);
+  }
+  const bool border = !(off < near);
+  if (__any_sync(0xffffffffu, border)) {
+    if (border) {
+      code = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) code |= kv4_code_fp64(x(i), m, d) << (4 * i);
+    }
+  }
+  meta = (__float_as_uint(d) >> 16) | mb;
+  // a value that is not finite makes its 64 NaN: 4 bits have no such value
+  const int lane = threadIdx.x & 31;
+  if (bad >> (lane & ~(RL - 1)) & ((RL == 32 ? 0u : 1u << RL) - 1u)) {
+    code = 0;
+    meta = 0x7FC00000u | (__float_as_uint(kKv4MinStep) >> 16);
+  }
+  return code;
+}
+
+// Four values of a row, fp32 or bf16 (16 or 8 bytes where the rows are aligned so).
+__device__ __forceinline__ void kv4_load4(const char* src, bool f32, bool wide, float (&x)[4]) {
+  if (f32) {
+    const float* v = reinterpret_cast<const float*>(src);
+    if (wide) {
+      const float4 w = *reinterpret_cast<const float4*>(v);
+      x[0] = w.x;
+      x[1] = w.y;
+      x[2] = w.z;
+      x[3] = w.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = v[i];
+    }
+  } else {
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(src);
+    if (wide) {
+      const uint2 w = *reinterpret_cast<const uint2*>(v);
+      x[0] = bf16lo_to_f32(w.x);
+      x[1] = bf16hi_to_f32(w.x);
+      x[2] = bf16lo_to_f32(w.y);
+      x[3] = bf16hi_to_f32(w.y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(v[i]);
+    }
+  }
 }
 
 template <int D>
-__global__ void __launch_bounds__(kKv4AppendThreads) kv4_append_kernel(const Kv4RowsParams p,
-                                                                      const __grid_constant__ Kv4Rope rope) {
-  constexpr int G = D / kKv4Group, J = D / 32, W = kKv4AppendThreads / 32, T = kKv4Tile / W;
-  __shared__ __align__(16) uint8_t codes[2][kKv4Tile][D];  // K, V
-  __shared__ uint32_t meta[2][G][kKv4Tile];
+__global__ void __launch_bounds__(kKv4AppendThreads, D == 64 ? 5 : 5) kv4_append_kernel(const Kv4RowsParams p,
+                                                                         const __grid_constant__ Kv4Rope rope) {
+  constexpr int G = D / kKv4Group, W = kKv4AppendThreads / 32;
+  constexpr int LR = D / 8, RW = 32 / LR, STEP = W * RW;  // lanes of a token, tokens of a warp, of the CTA
+  // a lane's 8 values are of one group of 64 (D = 64) or of two
+  constexpr int RL = D == 64 ? 8 : 16, NV = D == 64 ? 8 : 4, U = 8 / NV;
+  __shared__ __align__(16) uint8_t image[G * kKv4CellBytes];
+  __shared__ double turn_s[2][D / 2];  // cos, sin of the turn of STEP positions
   __shared__ float low[W][D], high[W][D];
   __shared__ int job_seq, job_page;
 
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int l = lane % LR, mine = warp * RW + lane / LR;  // this lane's place in its token; its token of STEP
   pdl_wait();
   pdl_launch_dependents();
   int b = blockIdx.x, pg = 0;
@@ -134,137 +229,155 @@ __global__ void __launch_bounds__(kKv4AppendThreads) kv4_append_kernel(const Kv4
   const long long base = static_cast<long long>(pg) * p.page;
   const int t0 = static_cast<int>(max(static_cast<long long>(pos), base) - base);
   const int t1 = static_cast<int>(min(static_cast<long long>(pos) + (row1 - row0), base + p.page) - base);
+  const int first = t0 / kKv4Tile * kKv4Tile;
   uint8_t* cells = p.pool + (static_cast<size_t>(id) * p.hkv + h) * (static_cast<size_t>(p.page / kKv4Tile) * G * kKv4CellBytes);
 
-  float lo_k[J], hi_k[J];
+  // the rows' bytes, from this lane's first token on; a token ahead of the work on it
+  const long long esize = p.is_f32 ? 4 : 2, row = row0 + (base + first + mine - pos);
+  const char* k_at = static_cast<const char*>(p.k) + (row * p.ld_k + static_cast<long long>(h) * D + 4 * l) * esize;
+  const char* v_at = static_cast<const char*>(p.v) + (row * p.ld_v + static_cast<long long>(h) * D + 4 * l) * esize;
+  const long long k_step = STEP * p.ld_k * esize, v_step = STEP * p.ld_v * esize, half = D / 2 * esize;
+  float k_in[2][4], v_in[2][4];
+  auto load = [&](int at) {
+    if (at >= t0 && at < t1) {
+      kv4_load4(k_at, p.is_f32, p.wide, k_in[0]);
+      kv4_load4(k_at + half, p.is_f32, p.wide, k_in[1]);
+      kv4_load4(v_at, p.is_f32, p.wide, v_in[0]);
+      kv4_load4(v_at + half, p.is_f32, p.wide, v_in[1]);
+    } else {  // its codes are not kept
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    lo_k[j] = INFINITY;
-    hi_k[j] = -INFINITY;
-  }
-  // the turn of this warp's first token, and that of the W positions to its next one
-  const int tile0 = t0 / kKv4Tile;
-  double cs[J / 2], sn[J / 2], cs_w[J / 2], sn_w[J / 2];
-  if (rope.on) {
-    const bool several = t1 - t0 > 1;
-    const double first = static_cast<double>(several ? base + tile0 * kKv4Tile + warp : base + t0);
-#pragma unroll
-    for (int j = 0; j < J / 2; ++j) {
-      const double turn = kv4_turn(rope, lane + 32 * j);
-      double u = first * turn;
-      u -= rint(u);
-      sincospi(2.0 * u, &sn[j], &cs[j]);
-      cs_w[j] = 1.0;
-      sn_w[j] = 0.0;
-      if (several) {
-        u = W * turn;
-        u -= rint(u);
-        sincospi(2.0 * u, &sn_w[j], &cs_w[j]);
-      }
+      for (int i = 0; i < 8; ++i) k_in[i / 4][i % 4] = v_in[i / 4][i % 4] = 0.f;
     }
-  }
-  for (int tile = tile0; tile * kKv4Tile < t1; ++tile) {
-    float in[T][2][J];
+    k_at += k_step;
+    v_at += v_step;
+  };
+  load(first + mine);
+
+  // the turn of this lane's first token; that of the STEP positions to its next one
+  const bool several = first + STEP < t1;
+  double cs[4], sn[4];
+  if (rope.on) {
+    if (several && threadIdx.x < D / 2) {
+      double u = STEP * kv4_turn(rope, threadIdx.x);
+      u -= rint(u);
+      kv4_cos_sin(u, turn_s[0][threadIdx.x], turn_s[1][threadIdx.x]);
+    }
+    const double at = static_cast<double>(base + first + mine);
 #pragma unroll
-    for (int i = 0; i < T; ++i) {
-      const int at = tile * kKv4Tile + warp + i * W;
-      if (at < t0 || at >= t1) continue;
-      const size_t row = static_cast<size_t>(row0 + (base + at - pos));
+    for (int i = 0; i < 4; ++i) {
+      double u = at * kv4_turn(rope, 4 * l + i);
+      u -= rint(u);
+      kv4_cos_sin(u, cs[i], sn[i]);
+    }
+    if (several) __syncthreads();
+  }
+  // least and largest keys of the lane's dims, as bf16 pairs: the rounding is monotone
+  __nv_bfloat162 lo_k[4], hi_k[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo_k[i] = __float2bfloat162_rn(INFINITY);
+    hi_k[i] = __float2bfloat162_rn(-INFINITY);
+  }
+
+  for (int tile = first; tile < t1; tile += kKv4Tile) {
+#pragma unroll 1
+    for (int t = mine; t < kKv4Tile; t += STEP) {
+      const int at = tile + t;
+      const bool fresh = at >= t0 && at < t1;
+      float k[8], f[8], v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        k[i] = k_in[i / 4][i % 4];
+        v[i] = v_in[i / 4][i % 4];
+      }
+      load(at + STEP);
+      auto turned = [&](int i) -> double {  // value i of the lane's eight keys
+        const int j = i & 3;
+        const double a = k[j], c = k[4 + j];
+        if (!rope.on) return i < 4 ? a : c;
+        return i < 4 ? a * cs[j] - c * sn[j] : c * cs[j] + a * sn[j];
+      };
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(turned(i));
+      if (fresh) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __nv_bfloat162 r = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          lo_k[i] = __hmin2(lo_k[i], r);
+          hi_k[i] = __hmax2(hi_k[i], r);
+        }
+      }
+      // the codes of the lane's two quads, and the (d, m) of their groups, into the cells' bytes
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        const size_t off = row * (which ? p.ld_v : p.ld_k) + static_cast<size_t>(h) * D + lane;
-        const void* src = which ? p.v : p.k;
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          in[i][which][j] = p.is_f32 ? static_cast<const float*>(src)[off + 32 * j]
-                                     : __bfloat162float(static_cast<const __nv_bfloat16*>(src)[off + 32 * j]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-      const int t = warp + i * W, at = tile * kKv4Tile + t;
-      if (at >= t0 && at < t1) {  // uniform in the warp
-        double x[J];
-        float f[J];
-        if (rope.on) {
-#pragma unroll
-          for (int j = 0; j < J / 2; ++j) {
-            const double a = in[i][0][j], c = in[i][0][j + J / 2];
-            x[j] = a * cs[j] - c * sn[j];
-            x[j + J / 2] = c * cs[j] + a * sn[j];
-          }
-#pragma unroll
-          for (int j = 0; j < J; ++j) f[j] = static_cast<float>(x[j]);
+        uint32_t quad[2], dm[2];
+        if (U == 1) {
+          const uint32_t c = which ? kv4_quantise<RL, 8>([&](int i) { return static_cast<double>(v[i]); }, v, dm[0])
+                                   : kv4_quantise<RL, 8>(turned, f, dm[0]);
+          quad[0] = c & 0xFFFFu;
+          quad[1] = c >> 16;
+          dm[1] = dm[0];
         } else {
 #pragma unroll
-          for (int j = 0; j < J; ++j) f[j] = in[i][0][j];
+          for (int u = 0; u < 2; ++u) {
+            float fu[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fu[i] = which ? v[4 * u + i] : f[4 * u + i];
+            quad[u] = which ? kv4_quantise<RL, 4>([&](int i) { return static_cast<double>(fu[i]); }, fu, dm[u])
+                            : kv4_quantise<RL, 4>([&](int i) { return turned(4 * u + i); }, fu, dm[u]);
+          }
         }
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const float r = round_bf16(f[j]);
-          lo_k[j] = fminf(lo_k[j], r);
-          hi_k[j] = fmaxf(hi_k[j], r);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          uint32_t c0, c1, dm;
-          if (rope.on) kv4_quantise<double>(x[2 * g], x[2 * g + 1], f[2 * g], f[2 * g + 1], c0, c1, dm);
-          else kv4_quantise<float>(f[2 * g], f[2 * g + 1], f[2 * g], f[2 * g + 1], c0, c1, dm);
-          codes[0][t][64 * g + lane] = static_cast<uint8_t>(c0);
-          codes[0][t][64 * g + 32 + lane] = static_cast<uint8_t>(c1);
-          if (lane == 0) meta[0][g][t] = dm;
-          const float v0 = in[i][1][2 * g], v1 = in[i][1][2 * g + 1];
-          kv4_quantise<float>(v0, v1, v0, v1, c0, c1, dm);
-          codes[1][t][64 * g + lane] = static_cast<uint8_t>(c0);
-          codes[1][t][64 * g + 32 + lane] = static_cast<uint8_t>(c1);
-          if (lane == 0) meta[1][g][t] = dm;
+        for (int u = 0; u < 2; ++u) {
+          const int dim = 4 * l + u * (D / 2), g = dim / kKv4Group, in = dim % kKv4Group;
+          uint8_t* cell = image + g * kKv4CellBytes;
+          const int to = which ? kv4_v_half(t, in / 4) : kv4_k_word(t, in / 8) + (in / 4 % 2) * 2;
+          *reinterpret_cast<uint16_t*>(cell + to) = static_cast<uint16_t>(quad[u]);
+          if (in == 0) *reinterpret_cast<uint32_t*>(cell + (which ? kKv4VMeta : kKv4KMeta) + kv4_meta(t)) = dm[u];
         }
       }
-      if (rope.on) {
+      if (rope.on && several) {
 #pragma unroll
-        for (int j = 0; j < J / 2; ++j) {
-          const double c = cs[j];
-          cs[j] = c * cs_w[j] - sn[j] * sn_w[j];
-          sn[j] = sn[j] * cs_w[j] + c * sn_w[j];
+        for (int i = 0; i < 4; ++i) {
+          const double c = cs[i], wc = turn_s[0][4 * l + i], ws = turn_s[1][4 * l + i];
+          cs[i] = c * wc - sn[i] * ws;
+          sn[i] = sn[i] * wc + c * ws;
         }
       }
     }
     __syncthreads();
-    uint8_t* cell0 = cells + static_cast<size_t>(tile) * G * kKv4CellBytes;
-    const int base_t = tile * kKv4Tile;
-    auto fresh = [&](int t) { return base_t + t >= t0 && base_t + t < t1; };
-    for (int e = threadIdx.x; e < G * 288; e += kKv4AppendThreads) {
-      const int g = e / 288, w = e % 288;
-      uint8_t* cell = cell0 + g * kKv4CellBytes;
-      if (w < 128) {  // a word of K codes: 8 dims of one token
-        const int t = w / 8, x = w % 8;
-        if (!fresh(t)) continue;
-        const uint2 bytes = *reinterpret_cast<const uint2*>(&codes[0][t][64 * g + 8 * x]);
-        *reinterpret_cast<uint32_t*>(cell + kv4_k_word(t, x)) = kv4_nibbles(bytes.x) | kv4_nibbles(bytes.y) << 16;
-      } else if (w < 256) {  // a word of V codes: 4 dims of two tokens
-        const int pr = (w - 128) / 16, x = (w - 128) % 16, t = 2 * pr;
-        const uint32_t a = kv4_nibbles(*reinterpret_cast<const uint32_t*>(&codes[1][t][64 * g + 4 * x]));
-        const uint32_t z = kv4_nibbles(*reinterpret_cast<const uint32_t*>(&codes[1][t + 1][64 * g + 4 * x]));
-        uint16_t* to = reinterpret_cast<uint16_t*>(cell + kv4_v_half(t, x));
-        if (fresh(t) && fresh(t + 1)) {
-          *reinterpret_cast<uint32_t*>(to) = a | z << 16;
-        } else {
-          if (fresh(t)) to[0] = static_cast<uint16_t>(a);
-          if (fresh(t + 1)) to[1] = static_cast<uint16_t>(z);
-        }
-      } else {
-        const int which = (w - 256) / 16, t = (w - 256) % 16;
-        if (fresh(t))
-          *reinterpret_cast<uint32_t*>(cell + (which ? kKv4VMeta : kKv4KMeta) + kv4_meta(t)) = meta[which][g][t];
+    uint8_t* cell0 = cells + static_cast<size_t>(tile / kKv4Tile) * G * kKv4CellBytes;
+    if (tile >= t0 && tile + kKv4Tile <= t1) {
+      for (int e = threadIdx.x; e < G * kKv4CellBytes / 16; e += kKv4AppendThreads)
+        reinterpret_cast<uint4*>(cell0)[e] = reinterpret_cast<const uint4*>(image)[e];
+    } else {  // the tokens beside the new ones stay: 2 bytes of K or V codes have one token, (d, m) 4
+      for (int e = threadIdx.x; e < G * kKv4CellBytes / 2; e += kKv4AppendThreads) {
+        const int o = e % (kKv4CellBytes / 2) * 2;
+        const int t = o < kKv4VCodes   ? o / 64 + o / 8 % 2 * 8
+                      : o < kKv4KMeta ? (o / 8 % 2) * 8 + (o / 16 % 4) * 2 + o / 2 % 2
+                                      : o % 64 / 8 + o / 4 % 2 * 8;
+        if (tile + t >= t0 && tile + t < t1)
+          reinterpret_cast<uint16_t*>(cell0)[e] = reinterpret_cast<const uint16_t*>(image)[e];
       }
     }
     __syncthreads();
   }
   if (!p.summary) return;
+  // the warp's tokens, then the warps
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    low[warp][lane + 32 * j] = lo_k[j];
-    high[warp][lane + 32 * j] = hi_k[j];
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = LR; o < 32; o <<= 1) {
+      lo_k[i] = __hmin2(lo_k[i], __shfl_xor_sync(0xffffffffu, lo_k[i], o));
+      hi_k[i] = __hmax2(hi_k[i], __shfl_xor_sync(0xffffffffu, hi_k[i], o));
+    }
+    if (lane < LR) {
+      const int dim = 4 * l + (i / 2) * (D / 2) + 2 * (i % 2);
+      low[warp][dim] = __low2float(lo_k[i]);
+      low[warp][dim + 1] = __high2float(lo_k[i]);
+      high[warp][dim] = __low2float(hi_k[i]);
+      high[warp][dim + 1] = __high2float(hi_k[i]);
+    }
   }
   __syncthreads();
   __nv_bfloat16* sm = p.summary + (static_cast<size_t>(id) * p.hkv + h) * 2 * D;
@@ -302,29 +415,36 @@ __device__ __forceinline__ void kv4_store8<__nv_bfloat16>(__nv_bfloat16* dst, co
   *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One CTA per (page of a sequence, kv head); a thread decodes 8 dims of one token of K and
-// of two tokens of V at a time and stores 8 values at once (rows 16-byte aligned).
+// One CTA per (page of a sequence, kv head).  128 threads have a word of K codes each (8 dims of
+// a token of the cell), 64 a pair of words of V (8 dims of two tokens), for every cell of the
+// page; 8 values are stored at once (rows 16-byte aligned).
+constexpr int kKv4GatherThreads = 192;
+
 template <int D, typename T>
-__global__ void __launch_bounds__(kKv4AppendThreads) kv4_gather_kernel(const Kv4RowsParams p) {
+__global__ void __launch_bounds__(kKv4GatherThreads) kv4_gather_kernel(const Kv4RowsParams p) {
   constexpr int G = D / kKv4Group;
   __shared__ int job_seq, job_page;
   const int h = blockIdx.y;
   pdl_wait();
   pdl_launch_dependents();
-  if (threadIdx.x < 32) {
-    int pg = 0;
-    const int b = kv4_find_job(p.cu, p.pos, p.rows, p.batch, p.page, blockIdx.x, pg);
-    if (threadIdx.x == 0) {
-      job_seq = b;
-      job_page = pg;
+  int b = blockIdx.x, pg = 0;
+  if (p.cu) {
+    if (threadIdx.x < 32) {
+      b = kv4_find_job(p.cu, p.pos, p.rows, p.batch, p.page, blockIdx.x, pg);
+      if (threadIdx.x == 0) {
+        job_seq = b;
+        job_page = pg;
+      }
     }
+    __syncthreads();
+    b = job_seq;
+    pg = job_page;
+    if (b < 0) return;
   }
-  __syncthreads();
-  const int b = job_seq, pg = job_page;
-  if (b < 0) return;
   int row0, row1;
   kv4_rows(p.cu, p.rows, b, row0, row1);
   const int pos = p.pos[b];
+  if (!p.cu) pg = max(pos, 0) / p.page;
   if (pos == -1 || row1 <= row0) return;
   const int id = pos < 0 ? -1 : kv4_page_id(p.table, p.max_pages, p.n_pages, b, pg);
   if (id < 0) {
@@ -334,39 +454,50 @@ __global__ void __launch_bounds__(kKv4AppendThreads) kv4_gather_kernel(const Kv4
   const long long base = static_cast<long long>(pg) * p.page;
   const int t0 = static_cast<int>(max(static_cast<long long>(pos), base) - base);
   const int t1 = static_cast<int>(min(static_cast<long long>(pos) + (row1 - row0), base + p.page) - base);
-  const uint8_t* cells = p.pool + (static_cast<size_t>(id) * p.hkv + h) * (static_cast<size_t>(p.page / kKv4Tile) * G * kKv4CellBytes);
-  T* kout = static_cast<T*>(const_cast<void*>(p.k));
-  T* vout = static_cast<T*>(const_cast<void*>(p.v));
-  const long long to_row = row0 + (base - pos);
-  const int tile0 = t0 / kKv4Tile, tiles = (t1 + kKv4Tile - 1) / kKv4Tile - tile0;
-  // per cell: 16 x 8 words of K, then 8 x 8 word pairs of V
-  for (int e = threadIdx.x; e < tiles * G * 192; e += kKv4AppendThreads) {
-    const int w = e % 192, g = e / 192 % G, tile = tile0 + e / (192 * G);
-    const uint8_t* cell = cells + (static_cast<size_t>(tile) * G + g) * kKv4CellBytes;
-    float x[8];
-    if (w < 128) {
-      const int t = w / 8, c = w % 8, at = tile * kKv4Tile + t;
-      if (at < t0 || at >= t1) continue;
+  const int tile0 = t0 / kKv4Tile, n_cells = ((t1 + kKv4Tile - 1) / kKv4Tile - tile0) * G;
+  const uint8_t* cells = p.pool + ((static_cast<size_t>(id) * p.hkv + h) * (p.page / kKv4Tile) + tile0) *
+                                      static_cast<size_t>(G * kKv4CellBytes);
+  const long long to_row = row0 + (base - pos) + tile0 * kKv4Tile;  // of the first tile's first token
+  const int lo = t0 - tile0 * kKv4Tile, hi = t1 - tile0 * kKv4Tile;
+  auto value = [](uint32_t code, uint32_t dm) {
+    return fmaf(static_cast<float>(code & 15u), bf16lo_to_f32(dm), bf16hi_to_f32(dm));
+  };
+  if (threadIdx.x < 128) {
+    const int t = threadIdx.x / 8, c = threadIdx.x % 8;
+    T* out = static_cast<T*>(const_cast<void*>(p.k)) + static_cast<size_t>(h) * D + 8 * c;
+#pragma unroll 4
+    for (int i = 0; i < n_cells; ++i) {
+      const uint8_t* cell = cells + static_cast<size_t>(i) * kKv4CellBytes;
       const uint32_t bits = *reinterpret_cast<const uint32_t*>(cell + kv4_k_word(t, c));
       const uint32_t dm = *reinterpret_cast<const uint32_t*>(cell + kKv4KMeta + kv4_meta(t));
+      const int at = i / G * kKv4Tile + t;
+      if (at < lo || at >= hi) continue;
+      float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((bits >> (4 * i)) & 15u), bf16lo_to_f32(dm), bf16hi_to_f32(dm));
-      kv4_store8<T>(kout + (to_row + at) * p.ld_k + static_cast<size_t>(h) * D + 64 * g + 8 * c, x);
-    } else {
-      const int pr = (w - 128) / 8, c = (w - 128) % 8;  // tokens 2 pr and 2 pr + 1, dims 8 c ..
+      for (int k = 0; k < 8; ++k) x[k] = value(bits >> (4 * k), dm);
+      kv4_store8<T>(out + (to_row + at) * p.ld_k + 64 * (i % G), x);
+    }
+  } else {
+    const int pr = (threadIdx.x - 128) / 8, c = threadIdx.x % 8;  // tokens 2 pr and 2 pr + 1
+    T* out = static_cast<T*>(const_cast<void*>(p.v)) + static_cast<size_t>(h) * D + 8 * c;
+#pragma unroll 2
+    for (int i = 0; i < n_cells; ++i) {
+      const uint8_t* cell = cells + static_cast<size_t>(i) * kKv4CellBytes;
       const uint2 bits = *reinterpret_cast<const uint2*>(cell + kv4_v_half(2 * pr, 2 * c));
+      uint32_t dm[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) dm[s] = *reinterpret_cast<const uint32_t*>(cell + kKv4VMeta + kv4_meta(2 * pr + s));
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int t = 2 * pr + s, at = tile * kKv4Tile + t;
-        if (at < t0 || at >= t1) continue;
-        const uint32_t dm = *reinterpret_cast<const uint32_t*>(cell + kKv4VMeta + kv4_meta(t));
-        const uint32_t q0 = bits.x >> (16 * s), q1 = bits.y >> (16 * s);
+        const int at = i / G * kKv4Tile + 2 * pr + s;
+        if (at < lo || at >= hi) continue;
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = fmaf(static_cast<float>((q0 >> (4 * i)) & 15u), bf16lo_to_f32(dm), bf16hi_to_f32(dm));
-          x[4 + i] = fmaf(static_cast<float>((q1 >> (4 * i)) & 15u), bf16lo_to_f32(dm), bf16hi_to_f32(dm));
+        for (int k = 0; k < 4; ++k) {
+          x[k] = value(bits.x >> (16 * s + 4 * k), dm[s]);
+          x[4 + k] = value(bits.y >> (16 * s + 4 * k), dm[s]);
         }
-        kv4_store8<T>(vout + (to_row + at) * p.ld_v + static_cast<size_t>(h) * D + 64 * g + 8 * c, x);
+        kv4_store8<T>(out + (to_row + at) * p.ld_v + 64 * (i % G), x);
       }
     }
   }

@@ -159,9 +159,11 @@ static int kv4_rows_call(bool append, const void* k, const void* v, int64_t ld_k
   p.max_pages = s.max_pages;
   p.n_pages = s.n_pages;
   p.is_f32 = f32;
+  const int64_t quad = f32 ? 16 : 8;
+  p.wide = aligned(k, quad) && aligned(v, quad) && ld_k % 4 == 0 && ld_v % 4 == 0;
   // a sequence of n rows touches at most n / page + 2 pages
   const int jobs = cu ? rows / s.page + 2 * s.batch : s.batch;
-  Kv4Launch l(dim3(jobs, s.hkv, 1), b2::kKv4AppendThreads, stream);
+  Kv4Launch l(dim3(jobs, s.hkv, 1), append ? b2::kKv4AppendThreads : b2::kKv4GatherThreads, stream);
   const b2::Kv4Rope& rope = kv4_rope(theta, s.head_dim, append ? flags : B2_KV4_NO_ROPE);
   const cudaError_t e = kv4_by_dim(s.head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
