@@ -454,12 +454,10 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
  * bound max_j sum_d max(q_jd lo_d, q_jd hi_d) over the kv head's q heads is largest (q
  * rotated; lo, hi the page's summary; in fp64).  The page of pos[b] is always listed, and
  * of two equal bounds the lower page goes first.  sel [batch][n_kv_heads][n_sel] ascending,
- * filled up with -1.  At most 16384 pages (max_len / page). */
-int b2_kv4_select_workspace_size(int batch, int n_kv_heads, int page, int max_len, size_t* bytes);
+ * filled up with -1.  At most 16384 pages (max_len / page); summary 16-byte aligned. */
 int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const int32_t* table, const int32_t* pos,
                   int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
-                  int max_pages, int n_pages, int max_len, float theta, void* workspace, size_t workspace_bytes,
-                  int flags, void* stream);
+                  int max_pages, int n_pages, int max_len, float theta, int flags, void* stream);
 
 /* Pages across the layers of a cache: pool [layers][n_pages][page_bytes], and summary
  * [layers][n_pages][summary_bytes] or null (bytes of a page, multiples of 16).  refs int32

@@ -73,9 +73,8 @@ SIGNATURES: dict[str, tuple] = {
     "b2_kv4_decode_workspace_size": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _c.POINTER(_c.c_size_t)]),
     "b2_kv4_decode": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                              _f32, _f32, _vp, _i64, _vp, _c.c_size_t, _i32, _vp]),
-    "b2_kv4_select_workspace_size": (_i32, [_i32, _i32, _i32, _i32, _c.POINTER(_c.c_size_t)]),
     "b2_kv4_select": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-                             _f32, _vp, _c.c_size_t, _i32, _vp]),
+                             _f32, _i32, _vp]),
     "b2_kv4_copy_pages": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _vp]),
     "b2_kv4_reorder_workspace_size": (_i32, [_i32, _i32, _i32, _c.POINTER(_c.c_size_t)]),
     "b2_kv4_reorder": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp,

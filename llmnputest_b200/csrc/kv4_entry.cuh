@@ -312,20 +312,9 @@ static int kv4_select_check(int page, int n_sel, int max_len, int* key_pages) {
   return B2_OK;
 }
 
-int b2_kv4_select_workspace_size(int batch, int n_kv_heads, int page, int max_len, size_t* bytes) {
-  if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
-  int pages;
-  const int st = kv4_select_check(page, 1, max_len, &pages);
-  if (st != B2_OK) return st;
-  if (batch < 1 || n_kv_heads < 1) return fail(B2_ERR_ARG, "empty batch");
-  *bytes = static_cast<size_t>(batch) * n_kv_heads * pages * sizeof(unsigned long long);
-  return B2_OK;
-}
-
 int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const int32_t* table, const int32_t* pos,
                   int32_t* sel, int n_sel, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page,
-                  int max_pages, int n_pages, int max_len, float theta, void* workspace, size_t workspace_bytes,
-                  int flags, void* stream) {
+                  int max_pages, int n_pages, int max_len, float theta, int flags, void* stream) {
   DevInfo di;
   int st = device_info(&di);
   if (st != B2_OK) return st;
@@ -339,9 +328,7 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   if (!(flags & B2_KV4_NO_ROPE) && !(theta > 0.f)) return fail(B2_ERR_ARG, "theta must be > 0");
   if (batch > 1 && ld_q < static_cast<int64_t>(n_q_heads) * head_dim)
     return fail(B2_ERR_ARG, "row stride below n_q_heads * head_dim");
-  const size_t need = static_cast<size_t>(batch) * n_kv_heads * pages * sizeof(unsigned long long);
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
-    return fail(B2_ERR_WORKSPACE, "kv4 select needs %zu bytes of 16-byte aligned workspace", need);
+  if (!aligned(summary, 16)) return fail(B2_ERR_ALIGN, "the summaries must be 16-byte aligned");
   b2::Kv4SelectParams p = {};
   p.q = q;
   p.ld_q = ld_q;
@@ -349,7 +336,6 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.table = table;
   p.pos = pos;
   p.sel = sel;
-  p.key = static_cast<unsigned long long*>(workspace);
   p.batch = batch;
   p.hq = n_q_heads;
   p.hkv = n_kv_heads;
@@ -359,21 +345,26 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.n_sel = n_sel;
   p.key_pages = pages;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
-  Kv4Launch l(dim3((pages + b2::kKv4ScorePages - 1) / b2::kKv4ScorePages, n_kv_heads, batch), b2::kKv4ScoreThreads,
-              stream);
-  cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
-    return cudaLaunchKernelEx(&l.cfg, b2::kv4_score_kernel<decltype(d)::value>, p, rope);
-  });
-  if (e != cudaSuccess) return cuda_fail(e, "kv4 select launch (bounds)");
+  // CTAs of a cluster: one per group of pages that its warps take at once, up to 8
+  const int group = b2::kKv4SelectThreads / 32 * (256 / head_dim);
+  p.ctas = std::max(1, std::min(8, (pages + group - 1) / group));
   const size_t smem = static_cast<size_t>(pages) * sizeof(unsigned long long);
-  if (smem > 40 * 1024) {
-    e = cudaFuncSetAttribute(b2::kv4_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kKv4MaxSelectPages * static_cast<int>(sizeof(unsigned long long)));
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(kv4 pick)");
-  }
-  Kv4Launch c(dim3(n_kv_heads, batch, 1), b2::kKv4PickThreads, stream, smem);
-  e = cudaLaunchKernelEx(&c.cfg, b2::kv4_pick_kernel, p);
-  if (e != cudaSuccess) return cuda_fail(e, "kv4 select launch (choice)");
+  const cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
+    auto kernel = b2::kv4_select_kernel<decltype(d)::value>;
+    static std::atomic<unsigned long long> ready{0};  // devices on which the kernel's attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(ready.load() >> dev & 1)) {
+      const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kKv4MaxSelectPages * static_cast<int>(sizeof(unsigned long long)));
+      if (r != cudaSuccess) return r;
+      ready.fetch_or(1ull << dev);
+    }
+    Kv4Launch l(dim3(p.ctas * n_kv_heads, batch, 1), b2::kKv4SelectThreads, stream, smem);
+    l.cluster(p.ctas);
+    return cudaLaunchKernelEx(&l.cfg, kernel, p, rope);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 select launch");
   return B2_OK;
 }
 
@@ -462,16 +453,9 @@ int b2_kv4_reorder(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t 
   p.batch = batch;
   p.max_pages = max_pages;
   p.page = page;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemcpyAsync(refs_out, refs, static_cast<size_t>(n_pages) * sizeof(int), cudaMemcpyDeviceToDevice, s);
-  if (e == cudaSuccess) e = cudaMemsetAsync(info, 0, 4 * sizeof(int), s);
-  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder set-up");
-  Kv4Launch a(dim3(batch, 1, 1), b2::kKv4CopyThreads, stream);
-  e = cudaLaunchKernelEx(&a.cfg, b2::kv4_reorder_rows_kernel, p);
-  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (rows)");
-  Kv4Launch f(dim3(1, 1, 1), b2::kKv4ScanThreads, stream);
-  e = cudaLaunchKernelEx(&f.cfg, b2::kv4_reorder_free_kernel, p);
-  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (free pages)");
+  Kv4Launch a(dim3(b2::kKv4PlanCtas, 1, 1), b2::kKv4PlanThreads, stream);
+  cudaError_t e = cudaLaunchKernelEx(&a.cfg, b2::kv4_reorder_plan_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (plan)");
   Kv4Launch c(dim3(kv4_copy_parts(p.data), batch, layers), b2::kKv4CopyThreads, stream);
   e = cudaLaunchKernelEx(&c.cfg, b2::kv4_reorder_fill_kernel, p);
   if (e != cudaSuccess) return cuda_fail(e, "kv4 reorder launch (copies)");

@@ -56,105 +56,122 @@ struct Kv4ReorderParams {
   int batch, max_pages, page;
 };
 
-// Row b's new entries, counts, and how many pages it lacks.  One CTA per row; refs_out holds
-// the old counts.
-__global__ void __launch_bounds__(kKv4CopyThreads) kv4_reorder_rows_kernel(const Kv4ReorderParams p) {
-  __shared__ int sh_first, sh_lack, sh_below;
-  const int b = blockIdx.x, tid = threadIdx.x, n_pages = p.data.n_pages;
+constexpr int kKv4ScanThreads = 1024;
+constexpr int kKv4PlanThreads = 512, kKv4PlanCtas = 8;
+
+// The new rows' entries and counts, and the lowest free pages in order, by one cluster (as one
+// grid after another, three launches and two copies, it took 13 us of the host's time):
+//   the counts copied; a warp per row takes the old row's holds back, the new one's up and
+//   counts what it lacks; every CTA counts the free pages of its share of the pool; then lists
+//   as many of them, from the lowest on, as all rows lack.
+__global__ void __launch_bounds__(kKv4PlanThreads) __cluster_dims__(kKv4PlanCtas, 1, 1)
+    kv4_reorder_plan_kernel(const Kv4ReorderParams p) {
+  constexpr int W = kKv4PlanThreads / 32;
+  __shared__ int warps[32], free_s[kKv4PlanCtas];
+  const int rank = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_pages = p.data.n_pages;
   pdl_wait();
   pdl_launch_dependents();
-  int par = p.parent[b];
-  if (par < -1 || par >= p.batch) {
-    if (tid == 0) record_error(kDevBadPosition);
-    par = -1;
-  }
-  if (tid == 0) {
-    sh_first = 1;
-    sh_lack = sh_below = 0;
-  }
-  __syncthreads();
-  if (par >= 0)
-    for (int i = tid; i < b; i += kKv4CopyThreads)
-      if (p.parent[i] == par) sh_first = 0;
-  __syncthreads();
-  const bool first = sh_first != 0;
-  const int len = par >= 0 ? max(p.lens[par], 0) : 0;
-  const int full = len / p.page;
-  const long long tokens = static_cast<long long>(len) + (p.reserve ? max(p.reserve[b], 0) : 0);
-  const long long want = (tokens + p.page - 1) / p.page;
-  const int* mine = p.table + static_cast<size_t>(b) * p.max_pages;
-  const int* theirs = p.table + static_cast<size_t>(max(par, 0)) * p.max_pages;
-  int* out = p.table_out + static_cast<size_t>(b) * p.max_pages;
-  int lack = 0, below = 0;
-  for (int j = tid; j < p.max_pages; j += kKv4CopyThreads) {
-    const int old = mine[j];
-    if (old >= 0 && old < n_pages) atomicSub(&p.refs_out[old], 1);
-    int id = par >= 0 && (first || j < full) ? theirs[j] : -1;
-    if (id >= n_pages) id = -1;
-    if (id >= 0) atomicAdd(&p.refs_out[id], 1);
-    else id = -1;
-    out[j] = id;
-    lack += id < 0 && j < want;
-    below += id < 0 && j < full;
-  }
-  if (lack) atomicAdd(&sh_lack, lack);
-  if (below) atomicAdd(&sh_below, below);
-  __syncthreads();
-  if (tid == 0) {
-    p.need[b] = sh_lack;
-    const bool copies = par >= 0 && !first && len % p.page != 0 && full < p.max_pages && theirs[full] >= 0 &&
-                        theirs[full] < n_pages;
-    p.copy[b] = copies ? 1 + sh_below : 0;
-    p.lens_out[b] = len;
-    if (want > p.max_pages) {
-      record_error(kDevNoPage);
-      atomicAdd(&p.info[2], static_cast<int>(min(want - p.max_pages, 0x7FFFFFFFll)));
+  for (int i = rank * kKv4PlanThreads + tid; i < n_pages; i += kKv4PlanCtas * kKv4PlanThreads) p.refs_out[i] = p.refs[i];
+  if (rank == 0 && tid < 4) p.info[tid] = 0;
+  cluster_sync_all();
+
+  for (int b = rank * W + warp; b < p.batch; b += kKv4PlanCtas * W) {
+    int par = p.parent[b];
+    if (par < -1 || par >= p.batch) {
+      if (lane == 0) record_error(kDevBadPosition);
+      par = -1;
+    }
+    bool taken = false;  // an earlier row goes on with the same one
+    if (par >= 0)
+      for (int i = lane; i < b; i += 32) taken |= p.parent[i] == par;
+    const bool first = !__any_sync(0xffffffffu, taken);
+    const int len = par >= 0 ? max(p.lens[par], 0) : 0;
+    const int full = len / p.page;
+    const long long tokens = static_cast<long long>(len) + (p.reserve ? max(p.reserve[b], 0) : 0);
+    const long long want = (tokens + p.page - 1) / p.page;
+    const int* mine = p.table + static_cast<size_t>(b) * p.max_pages;
+    const int* theirs = p.table + static_cast<size_t>(max(par, 0)) * p.max_pages;
+    int* out = p.table_out + static_cast<size_t>(b) * p.max_pages;
+    int lack = 0, below = 0;
+    for (int j = lane; j < p.max_pages; j += 32) {
+      const int old = mine[j];
+      int id = par >= 0 && (first || j < full) ? theirs[j] : -1;
+      if (id < 0 || id >= n_pages) id = -1;
+      if (old != id) {  // a row that goes on as it was changes no count
+        if (old >= 0 && old < n_pages) atomicSub(&p.refs_out[old], 1);
+        if (id >= 0) atomicAdd(&p.refs_out[id], 1);
+      }
+      out[j] = id;
+      lack += id < 0 && j < want;
+      below += id < 0 && j < full;
+    }
+    lack = __reduce_add_sync(0xffffffffu, lack);
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0) {
+      p.need[b] = lack;
+      const bool copies = par >= 0 && !first && len % p.page != 0 && full < p.max_pages && theirs[full] >= 0 &&
+                          theirs[full] < n_pages;
+      p.copy[b] = copies ? 1 + below : 0;
+      p.lens_out[b] = len;
+      if (want > p.max_pages) {
+        record_error(kDevNoPage);
+        atomicAdd(&p.info[2], static_cast<int>(min(want - p.max_pages, 0x7FFFFFFFll)));
+      }
     }
   }
-}
+  cluster_sync_all();
 
-constexpr int kKv4ScanThreads = 1024;
-
-// One CTA: sums of the rows' needs, and the lowest free pages in order.
-__global__ void __launch_bounds__(kKv4ScanThreads) kv4_reorder_free_kernel(const Kv4ReorderParams p) {
-  __shared__ int warps[32];
-  const int tid = threadIdx.x, n_pages = p.data.n_pages;
-  pdl_wait();
-  pdl_launch_dependents();
-  int total = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kKv4ScanThreads) {
-    const int b = b0 + tid, v = b < p.batch ? p.need[b] : 0;
+  // free pages of this CTA's share; the rows' needs in all (read past L1: others wrote them)
+  const int share = (n_pages + kKv4PlanCtas - 1) / kKv4PlanCtas;
+  const int lo = min(n_pages, rank * share), hi = min(n_pages, lo + share);
+  int mine = 0, free_here, total = 0;
+  for (int i = lo + tid; i < hi; i += kKv4PlanThreads) mine += __ldcg(&p.refs_out[i]) == 0;
+  kv4_block_before(mine, warps, free_here);
+  for (int b0 = 0; b0 < p.batch; b0 += kKv4PlanThreads) {
+    const int b = b0 + tid, v = b < p.batch ? __ldcg(&p.need[b]) : 0;
     int sum;
-    const int before = kv4_block_before(v, warps, sum);
-    if (b < p.batch) p.need[b] = total + before;
+    kv4_block_before(v, warps, sum);
     total += sum;
   }
-  int found = 0;
-  for (int i0 = 0; i0 < n_pages; i0 += 4 * kKv4ScanThreads) {
-    const int i = i0 + 4 * tid;
-    int free4 = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < n_pages && p.refs_out[i + e] == 0) free4 |= 1 << e;
-    int sum, rank = found + kv4_block_before(__popc(free4), warps, sum);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (free4 >> e & 1) {
-        if (rank < total) {
-          p.free_ids[rank] = i + e;
-          p.refs_out[i + e] = 1;
-        }
-        ++rank;
-      }
+  if (tid < kKv4PlanCtas) {
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&free_s[rank])), "r"(tid));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(free_here) : "memory");
+  }
+  cluster_sync_all();
+  int found = 0, all = 0;
+  for (int k = 0; k < kKv4PlanCtas; ++k) {
+    if (k < rank) found += free_s[k];
+    all += free_s[k];
+  }
+  for (int i0 = lo; i0 < hi && found < total; i0 += kKv4PlanThreads) {
+    const int i = i0 + tid;
+    const int is_free = i < hi && __ldcg(&p.refs_out[i]) == 0;
+    int sum;
+    const int at = found + kv4_block_before(is_free, warps, sum);
+    if (is_free && at < total) {
+      p.free_ids[at] = i;
+      p.refs_out[i] = 1;
+    }
     found += sum;
   }
-  if (tid == 0) {
-    p.totals[0] = total;
-    p.totals[1] = min(found, total);
-    p.info[0] = found - min(found, total);
-    if (found < total) {
-      record_error(kDevNoPage);
-      atomicAdd(&p.info[2], total - found);
+  if (rank == 0) {  // every CTA has summed the needs: they become the sums below each row
+    int below = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kKv4PlanThreads) {
+      const int b = b0 + tid, v = b < p.batch ? __ldcg(&p.need[b]) : 0;
+      int sum;
+      const int before = kv4_block_before(v, warps, sum);
+      if (b < p.batch) p.need[b] = below + before;
+      below += sum;
+    }
+    if (tid == 0) {
+      p.totals[0] = total;
+      p.totals[1] = min(all, total);
+      p.info[0] = all - min(all, total);
+      if (all < total) {
+        record_error(kDevNoPage);
+        atomicAdd(&p.info[2], total - all);
+      }
     }
   }
 }

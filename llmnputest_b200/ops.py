@@ -792,15 +792,9 @@ def kv4_decode(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: to
     return out
 
 
-def kv4_select_workspace_bytes(batch: int, n_kv_heads: int, page: int, max_len: int) -> int:
-    """Workspace of kv4_select."""
-    return _kv4_ws_bytes(torch.cuda.current_device(), "b2_kv4_select_workspace_size", batch, n_kv_heads, page, max_len)
-
-
 def kv4_select(q: torch.Tensor, summary: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, *, n_q_heads: int,
                n_kv_heads: int, head_dim: int, page: int, n_sel: int, theta: float | None = 10000.0,
-               max_len: int | None = None, out: torch.Tensor | None = None,
-               workspace: torch.Tensor | None = None) -> torch.Tensor:
+               max_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """The n_sel pages each kv head of each query attends to in a long cache, for
     kv4_decode's select (see b2_kv4_select): int32 [B, Hkv, n_sel] page indices, ascending,
     -1 behind them.
@@ -820,11 +814,8 @@ def kv4_select(q: torch.Tensor, summary: torch.Tensor, table: torch.Tensor, pos:
     chosen = _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
     if max_len is None:
         max_len = max_pages * page
-    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_select_workspace_size", batch, n_kv_heads, page, max_len),
-                 dev)
     _kv4_call(dev, "b2_kv4_select", q.data_ptr(), ld_q, near, table.data_ptr(), at, chosen, n_sel, batch, n_q_heads,
-              n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0, ws.data_ptr(), ws.numel(),
-              KV4_NO_ROPE if theta is None else 0)
+              n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0, KV4_NO_ROPE if theta is None else 0)
     return out
 
 

@@ -529,11 +529,10 @@ def test_captured_step_and_other_streams(ops):
     sel = torch.zeros(2, 2, 3, dtype=torch.int32, device="cuda")
     need = ops.kv4_decode_workspace_bytes(2, 10, 2, 64, 16, 16 * c.table.shape[1], 3)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
-    ws2 = torch.empty(ops.kv4_select_workspace_bytes(2, 2, 16, 16 * c.table.shape[1]), dtype=torch.uint8, device="cuda")
 
     def step():
         ops.kv4_append(kv[:, :128], kv[:, 128:], c.pool, c.dtable, pos, summary=c.summary, **c.heads)
-        ops.kv4_select(q, c.summary, c.dtable, pos, n_q_heads=10, page=16, n_sel=3, out=sel, workspace=ws2, **c.heads)
+        ops.kv4_select(q, c.summary, c.dtable, pos, n_q_heads=10, page=16, n_sel=3, out=sel, **c.heads)
         ops.kv4_decode(q, c.pool, c.dtable, pos, n_q_heads=10, select=sel, out=out, out_f32=True, workspace=ws,
                        **c.heads)
 

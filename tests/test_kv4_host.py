@@ -78,8 +78,7 @@ def test_calls_fail_cleanly_without_a_device():
     assert lib.b2_kv4_decode_workspace_size(1, 40, 8, 64, 64, 0, 256, ctypes.byref(n)) == -4
     assert lib.b2_kv4_decode(None, 2560, None, None, None, None, 0, 1, 40, 8, 64, 64, 4, 4, 256, 1e4, 0.125, None,
                              2560, None, 0, 0, None) == -4
-    assert lib.b2_kv4_select(None, 2560, None, None, None, None, 2, 1, 40, 8, 64, 64, 4, 4, 256, 1e4, None, 0, 0,
-                             None) == -4
+    assert lib.b2_kv4_select(None, 2560, None, None, None, None, 2, 1, 40, 8, 64, 64, 4, 4, 256, 1e4, 0, None) == -4
     assert lib.b2_kv4_copy_pages(None, 4608, None, 0, 1, 4, None, None, 1, None) == -4
     assert lib.b2_kv4_reorder(None, 4608, None, 0, 1, 4, None, None, None, None, None, 1, 4, 64, None, None, None,
                               None, None, 0, None) == -4
@@ -88,8 +87,6 @@ def test_calls_fail_cleanly_without_a_device():
 
 def test_workspace_sizes():
     lib, n = _native.lib(), ctypes.c_size_t()
-    assert lib.b2_kv4_select_workspace_size(2, 8, 64, 4096, ctypes.byref(n)) == 0 and n.value >= 2 * 8 * 64 * 8
-    assert lib.b2_kv4_select_workspace_size(2, 8, 64, 64 * 16385, ctypes.byref(n)) == -1
     assert lib.b2_kv4_reorder_workspace_size(4, 10, 100, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.b2_kv4_reorder_workspace_size(0, 10, 100, ctypes.byref(n)) == -1
     assert lib.b2_kv4_compact_workspace_size(100, ctypes.byref(n)) == 0 and n.value >= 1200
