@@ -12,7 +12,7 @@
 
 namespace {
 
-constexpr int kKv4MaxSelectPages = 16384;  // the keys of one (sequence, kv head) in 128 KB of shared memory
+constexpr int kKv4MaxSelectPages = 16384;  // 12 bytes of shared memory each: 192 KB
 
 struct Kv4Shape {
   int batch, hkv, head_dim, page, max_pages, n_pages;
@@ -345,10 +345,13 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.n_sel = n_sel;
   p.key_pages = pages;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
-  // CTAs of a cluster: one per group of pages that its warps take at once, up to 8
+  // CTAs of a cluster: one per group of pages that its warps take at once, up to 8, and no more
+  // than the GPU holds in all (two per SM: 16 sequences x 8 kv heads of up to 1024 pages in
+  // clusters of 8 came in 3.5 waves and took 32.6 us)
   const int group = b2::kKv4SelectThreads / 32 * (256 / head_dim);
-  p.ctas = std::max(1, std::min(8, (pages + group - 1) / group));
-  const size_t smem = static_cast<size_t>(pages) * sizeof(unsigned long long);
+  const long long pairs = static_cast<long long>(batch) * n_kv_heads;
+  p.ctas = static_cast<int>(std::max(1LL, std::min({8LL, static_cast<long long>((pages + group - 1) / group), 2LL * di.sms / pairs})));
+  const size_t smem = static_cast<size_t>(pages) * 12;
   const cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
     auto kernel = b2::kv4_select_kernel<decltype(d)::value>;
     static std::atomic<unsigned long long> ready{0};  // devices on which the kernel's attribute is set
@@ -356,7 +359,7 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
     cudaGetDevice(&dev);
     if (!(ready.load() >> dev & 1)) {
       const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kKv4MaxSelectPages * static_cast<int>(sizeof(unsigned long long)));
+                                                 kKv4MaxSelectPages * 12);
       if (r != cudaSuccess) return r;
       ready.fetch_or(1ull << dev);
     }

@@ -7,16 +7,18 @@
 // bounds are listed, in ascending order of the page; the page of the query's own position
 // is always among them, and of two equal bounds the lower page goes first.
 //
-// Which page is the n_sel-th turns on the last bit of two bounds, so q is turned and the
-// sums are taken in fp64; the summaries are bf16, so that every product is exact.
+// Which page is the n_sel-th may turn on the last bit of two bounds.  The bounds are summed in
+// fp32, with E, a bound on what that is off; where the last page taken and the first left out
+// are further apart than 2 E the choice is the exact one.  Where not (about one kv head in 300
+// of random keys; always with equal bounds), the pages within 2 E of the border are summed again in
+// fp64, with q turned in fp64 and the summaries bf16, every product exact, and chosen by that.
+// (In fp64 throughout the bounds of 512 pages of 8 kv heads took 4.6 us of 9.8, and those of
+// 16 sequences of up to 1024 pages 35 of 45.)
 //
 // A cluster per (sequence, kv head): its CTAs take every further group of pages, a warp
-// 256 / D pages at a time (D / 8 lanes a page, 8 dims each), and push the bounds, as integers
-// of the same order, into the first CTA's shared memory, which finds the n_sel-th by 8-bit
-// digits from the highest bit in which they differ, until a digit settles it (two or three
-// rounds of eight), and writes the pages in order.  One launch and no workspace; with the
-// bounds in a kernel of their own, a warp per page, and eight rounds, 512 pages of 8 kv heads
-// measured 21 us and 16 sequences of up to 1024 pages 41 us.
+// 256 / D pages at a time (D / 8 lanes a page, 8 dims each), and push the bounds into the first
+// CTA's shared memory, which finds the n_sel-th by 8-bit digits from the highest bit in which
+// they differ, until a digit settles it (two or three rounds), and writes the pages in order.
 #pragma once
 
 #include "kv4_cell.cuh"
@@ -36,33 +38,108 @@ struct Kv4SelectParams {
   int ctas;       // of a cluster
 };
 
-// a double as an unsigned integer of the same order, 1 or more; NaN and -inf are 1
+// Numbers as unsigned integers of the same order, 1 or more; NaN and -inf are 1.
+__device__ __forceinline__ unsigned kv4_key(float x) {
+  if (!(x > -INFINITY)) return 1;
+  const unsigned u = __float_as_uint(x);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
 __device__ __forceinline__ unsigned long long kv4_key(double x) {
   if (!(x > -INFINITY)) return 1;
   const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(x));
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ void st_dsmem_u64(uint32_t local_addr, uint32_t rank, unsigned long long v) {
-  uint32_t ra;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(local_addr), "r"(rank));
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ra), "l"(v) : "memory");
-}
-
 constexpr int kKv4SelectThreads = 256;
 
+// The need-th largest of n keys (0 < need < n): on return those whose bits from `shift` up are
+// above `at` are `need` - `left`, and of those at it the first `left` belong to them; `whole`
+// if those at it are `left`.
+struct Kv4Nth {
+  unsigned long long at;
+  int shift, left;
+  bool whole;
+};
+struct Kv4NthShared {
+  int hist[256], scan[kKv4SelectThreads / 32], digit, above, count;
+  unsigned long long diff;
+};
+template <typename F>
+__device__ __forceinline__ Kv4Nth kv4_nth(const F& key, int n, int need, Kv4NthShared& sh) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) sh.diff = 0;
+  __syncthreads();
+  const unsigned long long k0 = key(0);
+  unsigned long long d = 0;
+  for (int i = tid; i < n; i += kKv4SelectThreads) d |= key(i) ^ k0;
+  const unsigned hi = __reduce_or_sync(0xffffffffu, static_cast<unsigned>(d >> 32));
+  const unsigned lo = __reduce_or_sync(0xffffffffu, static_cast<unsigned>(d));
+  if (lane == 0 && (hi | lo)) atomicOr(&sh.diff, static_cast<unsigned long long>(hi) << 32 | lo);
+  __syncthreads();
+  Kv4Nth r;
+  r.shift = sh.diff ? 64 - __clzll(sh.diff) : 0;
+  r.at = r.shift < 64 ? k0 >> r.shift : 0;  // the common beginning
+  r.left = need;
+  r.whole = false;
+  while (r.shift > 0 && !r.whole) {
+    const int bits = min(8, r.shift);
+    sh.hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kKv4SelectThreads) {
+      const unsigned long long k = key(i);
+      if ((r.shift < 64 ? k >> r.shift : 0) == r.at) atomicAdd(&sh.hist[k >> (r.shift - bits) & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // digits from the top: the one at which the count from above reaches `left`
+    const int mine = sh.hist[255 - tid];
+    int s = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    if (lane == 31) sh.scan[warp] = s;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) s += sh.scan[w];
+    if (s >= r.left && s - mine < r.left) {
+      sh.digit = 255 - tid;
+      sh.above = s - mine;
+      sh.count = mine;
+    }
+    __syncthreads();
+    r.shift -= bits;
+    r.at = r.at << bits | static_cast<unsigned>(sh.digit);
+    r.left -= sh.above;
+    r.whole = sh.count == r.left;
+  }
+  return r;
+}
+
+// 8 bf16 pairs as they are stored (lo and hi of a lane's dims)
+struct Kv4Near {
+  uint4 lo, hi;
+};
+
 template <int D>
-__global__ void __launch_bounds__(kKv4SelectThreads) kv4_select_kernel(const Kv4SelectParams p,
+__global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const Kv4SelectParams p,
                                                                       const __grid_constant__ Kv4Rope rope) {
   constexpr int LR = D / 8, RW = 32 / LR, W = kKv4SelectThreads / 32;
-  extern __shared__ unsigned long long keys[];  // the first CTA's are used
-  __shared__ __align__(16) double q[kKv4MaxGroup][D];
+  extern __shared__ __align__(16) unsigned long long exact[];  // [key_pages], then the fp32 bounds (the first CTA's)
+  float* const bound = reinterpret_cast<float*>(exact + p.key_pages);
+  __shared__ __align__(16) float q_s[kKv4MaxGroup][D];
   __shared__ double turn_s[2][D / 2];
-  __shared__ int hist[256], scan[W], sh_digit, sh_above, sh_count;
-  __shared__ unsigned long long sh_diff;
+  __shared__ float size[W];
+  __shared__ unsigned most;  // the largest sum_d qa |lo or hi| of a page, its bits (the first CTA's)
+  __shared__ int n_close;
+  __shared__ float in_least[W], out_most[W];
+  __shared__ Kv4NthShared nth_s;
   const int rank = blockIdx.x % p.ctas, kvh = blockIdx.x / p.ctas, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = p.hq / p.hkv;
-  if (p.ctas > 1) cluster_arrive_relaxed();  // waited for before anything is pushed
+  if (tid == 0) most = 0;
+  if (p.ctas > 1) {
+    __syncthreads();
+    cluster_arrive_release();  // waited for before anything is pushed
+  }
   pdl_wait();
   pdl_launch_dependents();
   int* sel = p.sel + (static_cast<size_t>(b) * p.hkv + kvh) * p.n_sel;
@@ -77,142 +154,205 @@ __global__ void __launch_bounds__(kKv4SelectThreads) kv4_select_kernel(const Kv4
   }
   const int n = pos / p.page + 1;  // pages; the last is chosen without a bound
   const int need = p.n_sel - 1;    // of the n - 1 others
-  if (need < n - 1 && need > 0) {
-    // ---- q turned to pos
-    if (rope.on) {
-      for (int i = tid; i < D / 2; i += kKv4SelectThreads) {
-        double u = static_cast<double>(pos) * kv4_turn(rope, i);
-        u -= rint(u);
-        kv4_cos_sin(u, turn_s[0][i], turn_s[1][i]);
+  if (need >= n - 1 || need == 0) {
+    if (rank == 0)
+      for (int i = tid; i < p.n_sel; i += kKv4SelectThreads) {
+        const int pg = need == 0 ? n - 1 : i;
+        if (pg < n && kv4_page_id(p.table, p.max_pages, p.n_pages, b, pg) < 0) record_error(kDevBadPosition);
+        sel[i] = pg < n ? pg : -1;
       }
-      __syncthreads();
-    }
-    for (int e = tid; e < grp * (D / 2); e += kKv4SelectThreads) {
-      const int j = e / (D / 2), i = e % (D / 2);
-      const float* src = p.q + static_cast<size_t>(b) * p.ld_q + static_cast<size_t>(kvh * grp + j) * D;
-      const double a = src[i], z = src[i + D / 2];
-      const double c = rope.on ? turn_s[0][i] : 1.0, s = rope.on ? turn_s[1][i] : 0.0;
-      q[j][i] = a * c - z * s;
-      q[j][i + D / 2] = z * c + a * s;
-    }
-    __syncthreads();
     if (p.ctas > 1) cluster_wait_acquire();
-    // ---- the bounds
-    const uint32_t keys_s = smem_u32(keys);
-    const int l = lane % LR, sub = lane / LR;
-    for (int pg0 = (rank * W + warp) * RW; pg0 < n - 1; pg0 += p.ctas * W * RW) {
-      const int pg = pg0 + sub;
-      const bool in = pg < n - 1;
-      const int id = in ? kv4_page_id(p.table, p.max_pages, p.n_pages, b, pg) : -1;
-      double lo[8], hi[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.0;
-      if (id >= 0) {
-        const __nv_bfloat16* sm = p.summary + (static_cast<size_t>(id) * p.hkv + kvh) * 2 * D + 8 * l;
-        const uint4 a = *reinterpret_cast<const uint4*>(sm), z = *reinterpret_cast<const uint4*>(sm + D);
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, zw[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[2 * i] = bf16lo_to_f32(aw[i]);
-          lo[2 * i + 1] = bf16hi_to_f32(aw[i]);
-          hi[2 * i] = bf16lo_to_f32(zw[i]);
-          hi[2 * i + 1] = bf16hi_to_f32(zw[i]);
-        }
-      }
-      double best = -INFINITY;
-      for (int j = 0; j < grp; ++j) {
-        const double2* x2 = reinterpret_cast<const double2*>(&q[j][8 * l]);
-        double s = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const double2 x = x2[i];
-          s = fma(x.x, x.x > 0.0 ? hi[2 * i] : lo[2 * i], s);
-          s = fma(x.y, x.y > 0.0 ? hi[2 * i + 1] : lo[2 * i + 1], s);
-        }
-#pragma unroll
-        for (int o = LR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        best = fmax(best, s);
-      }
-      if (in && l == 0) {
-        if (id < 0) record_error(kDevBadPosition);
-        const unsigned long long k = id < 0 ? 0ull : kv4_key(best);
-        if (p.ctas > 1) st_dsmem_u64(keys_s + pg * 8, 0, k);
-        else keys[pg] = k;
-      }
-    }
-    if (p.ctas > 1) cluster_sync_all();
-  } else if (p.ctas > 1) {
-    cluster_wait_acquire();
-  }
-  if (rank != 0) return;  // nothing reads this CTA's shared memory
-  if (need >= n - 1) {    // every page
-    for (int i = tid; i < p.n_sel; i += kKv4SelectThreads) {
-      if (i < n && kv4_page_id(p.table, p.max_pages, p.n_pages, b, i) < 0) record_error(kDevBadPosition);
-      sel[i] = i < n ? i : -1;
-    }
     return;
   }
+  const int l = lane % LR, sub = lane / LR;
+  auto find = [&](int pg) { return pg < n - 1 ? kv4_page_id(p.table, p.max_pages, p.n_pages, b, pg) : -1; };
+  auto load = [&](int id, Kv4Near& x) {  // this lane's part of a page's summary
+    x.lo = x.hi = make_uint4(0, 0, 0, 0);
+    if (id >= 0) {
+      const __nv_bfloat16* sm = p.summary + (static_cast<size_t>(id) * p.hkv + kvh) * 2 * D + 8 * l;
+      x.lo = *reinterpret_cast<const uint4*>(sm);
+      x.hi = *reinterpret_cast<const uint4*>(sm + D);
+    }
+  };
+  // ---- the first pages' summaries set out; q turned to pos
+  const int step = p.ctas * W * RW;
+  int pg = (rank * W + warp) * RW + sub;
+  Kv4Near x;
+  int id = find(pg), id_next = find(pg + step);
+  load(id, x);
+  if (rope.on) {
+    for (int i = tid; i < D / 2; i += kKv4SelectThreads) {
+      double u = static_cast<double>(pos) * kv4_turn(rope, i);
+      u -= rint(u);
+      kv4_cos_sin(u, turn_s[0][i], turn_s[1][i]);
+    }
+    __syncthreads();
+  }
+  // value i or i + D / 2 of head j, turned
+  auto turned = [&](int j, int i, bool second) -> double {
+    const float* src = p.q + static_cast<size_t>(b) * p.ld_q + static_cast<size_t>(kvh * grp + j) * D;
+    const double a = src[i], z = src[i + D / 2];
+    if (!rope.on) return second ? z : a;
+    const double c = turn_s[0][i], s = turn_s[1][i];
+    return second ? z * c + a * s : a * c - z * s;
+  };
+  for (int e = tid; e < grp * (D / 2); e += kKv4SelectThreads) {
+    const int j = e / (D / 2), i = e % (D / 2);
+    q_s[j][i] = static_cast<float>(turned(j, i, false));
+    q_s[j][i + D / 2] = static_cast<float>(turned(j, i, true));
+  }
+  __syncthreads();
+  // this lane's dims of every head, and the largest of the heads
+  float q[kKv4MaxGroup][8], qa[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    qa[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kKv4MaxGroup; ++j) {
+      q[j][i] = j < grp ? q_s[j][8 * l + i] : 0.f;
+      qa[i] = fmaxf(qa[i], fabsf(q[j][i]));
+    }
+  }
+  if (p.ctas > 1) cluster_wait_acquire();
+  // ---- the bounds in fp32: max(q lo, q hi) = q mid + |q| half
+  const uint32_t bound_s = smem_u32(bound);
+  float top = 0.f;
+  while (__any_sync(0xffffffffu, pg < n - 1)) {
+    Kv4Near y;
+    load(id_next, y);
+    const int id_after = find(pg + 2 * step);
+    float mid[8], half[8], s[kKv4MaxGroup], all = 0.f;  // all: of the products' sizes
+    const uint32_t lw[4] = {x.lo.x, x.lo.y, x.lo.z, x.lo.w}, hw[4] = {x.hi.x, x.hi.y, x.hi.z, x.hi.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float lo = i % 2 ? bf16hi_to_f32(lw[i / 2]) : bf16lo_to_f32(lw[i / 2]);
+      const float hi = i % 2 ? bf16hi_to_f32(hw[i / 2]) : bf16lo_to_f32(hw[i / 2]);
+      mid[i] = 0.5f * hi + 0.5f * lo;
+      half[i] = 0.5f * hi - 0.5f * lo;
+      all = fmaf(qa[i], fabsf(mid[i]) + fabsf(half[i]), all);
+    }
+#pragma unroll
+    for (int j = 0; j < kKv4MaxGroup; ++j) {
+      s[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[j] = fmaf(q[j][i], mid[i], fmaf(fabsf(q[j][i]), half[i], s[j]));
+    }
+    float best = -INFINITY;
+#pragma unroll
+    for (int o = LR / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    top = all <= top ? top : all < INFINITY ? all : INFINITY;  // NaN too: nothing is then decided in fp32
+#pragma unroll
+    for (int j = 0; j < kKv4MaxGroup; ++j)
+      if (j < grp) {
+#pragma unroll
+        for (int o = LR / 2; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+        best = fmaxf(best, s[j]);
+      }
+    if (pg < n - 1 && l == 0) {
+      if (id < 0) {
+        record_error(kDevBadPosition);
+        best = -INFINITY;
+      }
+      if (p.ctas > 1) st_dsmem_f32(bound_s + pg * 4, 0, best);
+      else bound[pg] = best;
+    }
+    x = y;
+    id = id_next;
+    id_next = id_after;
+    pg += step;
+  }
+  top = warp_max(top);
+  if (lane == 0) size[warp] = top;
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, size[w]);
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(&most)));
+    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(to), "r"(__float_as_uint(top)) : "memory");
+  }
+  if (p.ctas > 1) cluster_sync_all();
+  else __syncthreads();
+  if (rank != 0) return;  // nothing reads this CTA's shared memory
+
+  // ---- the need largest bounds
   if (tid == 0) {
     if (kv4_page_id(p.table, p.max_pages, p.n_pages, b, n - 1) < 0) record_error(kDevBadPosition);
     sel[need] = n - 1;
-    sh_diff = 0;
   }
-  if (need == 0) return;
-  __syncthreads();
-  // ---- the highest bit in which two bounds differ
-  {
-    unsigned long long d = 0;
-    const unsigned long long k0 = keys[0];
-    for (int i = tid; i < n - 1; i += kKv4SelectThreads) d |= keys[i] ^ k0;
-    const unsigned hi = __reduce_or_sync(0xffffffffu, static_cast<unsigned>(d >> 32));
-    const unsigned lo = __reduce_or_sync(0xffffffffu, static_cast<unsigned>(d));
-    if (lane == 0 && (hi | lo)) atomicOr(&sh_diff, static_cast<unsigned long long>(hi) << 32 | lo);
+  auto key = [&](int i) { return static_cast<unsigned long long>(kv4_key(bound[i])); };
+  Kv4Nth t = kv4_nth(key, n - 1, need, nth_s);
+  // E: every lane's 16 products and the log2(D / 8) sums over lanes are rounded by 2^-24 of the
+  // sizes' sum at most, and so are q, mid and half; the sizes' own sum is fp32 too
+  const float off = __uint_as_float(most) * (28 * 5.9604644775390625e-8f);
+  float least = INFINITY, first_out = -INFINITY;  // of those taken, of those left out
+  for (int i = tid; i < n - 1; i += kKv4SelectThreads) {
+    if ((key(i) >> t.shift) >= t.at) least = fminf(least, bound[i]);
+    else first_out = fmaxf(first_out, bound[i]);
+  }
+  least = -warp_max(-least);
+  first_out = warp_max(first_out);
+  if (lane == 0) {
+    in_least[warp] = least;
+    out_most[warp] = first_out;
   }
   __syncthreads();
-  // ---- the need-th largest: of the keys that begin as `at` does down to bit `shift`, `left` are
-  // to be taken, the larger ones all
-  unsigned long long at = keys[0];
-  int shift = sh_diff ? 64 - __clzll(sh_diff) : 0, left = need;
-  at = shift < 64 ? at >> shift : 0;  // the common beginning
-  while (shift > 0) {
-    const int bits = min(8, shift);
-    hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n - 1; i += kKv4SelectThreads) {
-      const unsigned long long k = keys[i];
-      if ((shift < 64 ? k >> shift : 0) == at) atomicAdd(&hist[k >> (shift - bits) & ((1 << bits) - 1)], 1);
-    }
-    __syncthreads();
-    // digits from the top: the one at which the count from above reaches `left`
-    const int mine = hist[255 - tid];
-    int s = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += v;
-    }
-    if (lane == 31) scan[warp] = s;
+  for (int w = 0; w < W; ++w) {
+    least = fminf(least, in_least[w]);
+    first_out = fmaxf(first_out, out_most[w]);
+  }
+  const bool sure = t.whole && least - first_out > 2.f * off;  // false where off is not finite
+  if (!sure) {
+    // ---- again for those within 2 E of the border, in fp64: a warp a page
+    if (tid == 0) n_close = 0;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) s += scan[w];
-    if (s >= left && s - mine < left) {
-      sh_digit = 255 - tid;
-      sh_above = s - mine;
-      sh_count = mine;
+    int* const close = reinterpret_cast<int*>(bound);  // their list takes the bounds' place, from below
+    for (int i0 = 0; i0 < n - 1; i0 += kKv4SelectThreads) {
+      const int i = i0 + tid;
+      const float v = i < n - 1 ? bound[i] : 0.f;
+      const bool in = v > least + 2.f * off, out = v < least - 2.f * off;
+      if (i < n - 1) exact[i] = in ? ~0ull : 0ull;
+      __syncthreads();  // these bounds have been read
+      if (i < n - 1 && !in && !out) close[atomicAdd(&n_close, 1)] = i;
+      __syncthreads();
+    }
+    for (int c = warp; c < n_close; c += W) {
+      const int i = close[c], page = kv4_page_id(p.table, p.max_pages, p.n_pages, b, i);
+      unsigned long long k = 1;
+      if (page >= 0) {
+        const __nv_bfloat16* sm = p.summary + (static_cast<size_t>(page) * p.hkv + kvh) * 2 * D;
+        double best = -INFINITY;
+        for (int j = 0; j < grp; ++j) {
+          double s = 0.0;
+          for (int d = lane; d < D / 2; d += 32)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const double v = turned(j, d, e);
+              s = fma(v, static_cast<double>(__bfloat162float(sm[(v > 0.0 ? D : 0) + d + e * (D / 2)])), s);
+            }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          best = fmax(best, s);
+        }
+        k = min(kv4_key(best), ~0ull - 1);
+      }
+      if (lane == 0) exact[i] = k;
     }
     __syncthreads();
-    shift -= bits;
-    at = at << bits | static_cast<unsigned>(sh_digit);
-    left -= sh_above;
-    if (sh_count == left) break;  // every key that begins so is taken
+    t = kv4_nth([&](int i) { return exact[i]; }, n - 1, need, nth_s);
   }
   // ---- in order: every thread a run of pages; above `at` all, at it the first `left`
   const int per = (n - 1 + kKv4SelectThreads - 1) / kKv4SelectThreads;
   const int i0 = min(n - 1, tid * per), i1 = min(n - 1, i0 + per);
+  auto place = [&](int i) {
+    const unsigned long long k = sure ? key(i) : exact[i];
+    return t.shift < 64 ? k >> t.shift : 0ull;
+  };
   int above = 0, equal = 0;
   for (int i = i0; i < i1; ++i) {
-    const unsigned long long k = shift < 64 ? keys[i] >> shift : 0;
-    above += k > at;
-    equal += k == at;
+    above += place(i) > t.at;
+    equal += place(i) == t.at;
   }
   int both = above | (equal << 16), s = both;  // 16 bits each (n <= 16384)
 #pragma unroll
@@ -221,16 +361,16 @@ __global__ void __launch_bounds__(kKv4SelectThreads) kv4_select_kernel(const Kv4
     if (lane >= o) s += v;
   }
   __syncthreads();
-  if (lane == 31) scan[warp] = s;
+  if (lane == 31) nth_s.scan[warp] = s;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) s += scan[w];
+  for (int w = 0; w < warp; ++w) s += nth_s.scan[w];
   s -= both;
   int gt = s & 0xFFFF, eq = s >> 16;
   for (int i = i0; i < i1; ++i) {
-    const unsigned long long k = shift < 64 ? keys[i] >> shift : 0;
-    if (k > at || (k == at && eq < left)) sel[gt + min(eq, left)] = i;
-    gt += k > at;
-    eq += k == at;
+    const unsigned long long k = place(i);
+    if (k > t.at || (k == t.at && eq < t.left)) sel[gt + min(eq, t.left)] = i;
+    gt += k > t.at;
+    eq += k == t.at;
   }
 }
 
