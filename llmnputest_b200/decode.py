@@ -17,6 +17,8 @@ fp32; GEMV inputs are bf16 as in the reference.  Weights are the raw q4nx tiles,
 resident on the device; the step is captured in one CUDA graph.  Batches of 9
 and more run the projections on the tcgen05 GEMM (b2_q4_gemm / _swiglu_gemm, the
 norms fused into their x pre-pass: b2_q4_gemm_rmsnorm / _swiglu_gemm_rmsnorm).
+With kv_cache="kv4" K and V are kept in 4 bits in pages (llmnputest_b200.kv4) and attention is
+two calls, b2_kv4_append and b2_kv4_decode.
 
 The reference never ran a granite token loop (README.md:299-301); this module
 is the composition its layer design estimates (granite_layer.py:158-164).
@@ -31,6 +33,7 @@ import torch
 
 from . import ops
 from .format import Q4_TILE_BYTES, Q8_TILE_BYTES, TILE_K, TILE_ROWS
+from .kv4 import Kv4Cache
 
 
 @dataclass(frozen=True)
@@ -86,7 +89,12 @@ class Q4Decoder:
     """Resident weights, KV cache and buffers for batched decode; `step()` is graph-capturable."""
 
     def __init__(self, cfg: DecoderConfig, batch: int, ctx_max: int, device=None, seed: int = 0,
-                 weights: dict | None = None, gemm_min_batch: int = 9, pack_gemm: bool = True):
+                 weights: dict | None = None, gemm_min_batch: int = 9, pack_gemm: bool = True,
+                 kv_cache: str = "bf16", kv_page: int = 64):
+        """kv_cache: "bf16", dense caches of ctx_max positions; "kv4", 4-bit pages of kv_page
+        tokens (`cache`, a Kv4Cache with pages for ctx_max positions of every sequence)."""
+        if kv_cache not in ("bf16", "kv4"):
+            raise ValueError(f"kv_cache must be 'bf16' or 'kv4', got {kv_cache!r}")
         self.cfg = cfg
         self.batch = batch
         self.ctx_max = ctx_max
@@ -103,10 +111,20 @@ class Q4Decoder:
         if weights is None:
             weights = self._synthetic(seed)
         self.w = weights
-        # KV cache per layer: [B][Hkv][ctx_max][D] bf16
-        kv_shape = (batch, c.n_kv_heads, ctx_max, c.head_dim)
-        self.k_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
-        self.v_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
+        self.cache = None
+        if kv_cache == "kv4":
+            pages = -(-ctx_max // kv_page)
+            self.cache = Kv4Cache(c.n_layers, batch * pages, c.n_kv_heads, c.head_dim, batch, pages, kv_page, dev)
+            self.cache.reserve(ctx_max)
+            ws = ops.kv4_decode_workspace_bytes(batch, c.n_heads, c.n_kv_heads, c.head_dim, kv_page, ctx_max)
+            self.attn_ws = torch.empty(max(ws, 16), dtype=torch.uint8, device=dev)
+        else:
+            # KV cache per layer: [B][Hkv][ctx_max][D] bf16
+            kv_shape = (batch, c.n_kv_heads, ctx_max, c.head_dim)
+            self.k_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
+            self.v_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
+            ws = ops.gqa_decode_workspace_bytes(batch, c.n_heads, c.n_kv_heads, c.head_dim, ctx_max)
+            self.attn_ws = torch.empty(max(ws, 1), dtype=torch.uint8, device=dev)
         # activations
         self.x_in = torch.zeros(batch, c.hidden, dtype=torch.float32, device=dev)
         self.resid = torch.zeros(batch, c.hidden, dtype=torch.float32, device=dev)
@@ -116,8 +134,6 @@ class Q4Decoder:
         self.h = torch.zeros(batch, c.intermediate, dtype=torch.bfloat16, device=dev)
         self.logits = torch.zeros(batch, c.vocab, dtype=torch.float32, device=dev)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
-        ws = ops.gqa_decode_workspace_bytes(batch, c.n_heads, c.n_kv_heads, c.head_dim, ctx_max)
-        self.attn_ws = torch.empty(max(ws, 1), dtype=torch.uint8, device=dev)
         # batches of gemm_min_batch and more run the projections on the tcgen05 GEMM
         self.use_gemm = batch >= gemm_min_batch
         if self.use_gemm:
@@ -163,19 +179,13 @@ class Q4Decoder:
         wait on the preceding kernel).
         """
         c = self.cfg
-        d = c.head_dim
-        qd = c.n_heads * d
-        kd = c.n_kv_heads * d
         self.resid.copy_(self.x_in)
         if self.use_gemm:
             return self._step_gemm()
         for li, L in enumerate(self.w["layers"]):
             ops.gemv_rmsnorm(L["qkv"], self.nt_qkv, self.kt_h, self.resid, L["attn_norm"], c.rms_eps, out=self.qkv,
                              prefetch=prefetch)
-            ops.gqa_decode(self.qkv[:, :qd], self.qkv[:, qd:qd + kd], self.qkv[:, qd + kd:],
-                           self.k_cache[li], self.v_cache[li], self.pos, n_q_heads=c.n_heads,
-                           n_kv_heads=c.n_kv_heads, theta=c.rope_theta, scale=d ** -0.5, max_len=self.ctx_max,
-                           out=self.attn, workspace=self.attn_ws, prefetch_kv=prefetch)
+            self._attend(li, prefetch)
             ops.q4_gemv(L["o"], self.nt_h, self.kt_q, self.attn, out=self.resid, accumulate=True, prefetch=prefetch)
             ops.swiglu_gemv_rmsnorm(L["gate"], L["up"], self.nt_i, self.kt_h, self.resid, L["mlp_norm"], c.rms_eps,
                                     out=self.h, prefetch=prefetch)
@@ -184,12 +194,24 @@ class Q4Decoder:
                          out=self.logits, prefetch=prefetch, q8=True)
         return self.logits
 
+    def _attend(self, li: int, prefetch: bool) -> None:
+        """attn = layer li's attention on the rows of qkv, whose k and v join its cache at `pos`."""
+        c, d = self.cfg, self.cfg.head_dim
+        qd, kd = c.n_heads * d, c.n_kv_heads * d
+        q, k, v = self.qkv[:, :qd], self.qkv[:, qd:qd + kd], self.qkv[:, qd + kd:]
+        if self.cache is not None:
+            self.cache.append(li, k, v, self.pos, theta=c.rope_theta)
+            self.cache.decode(li, q, self.pos, n_q_heads=c.n_heads, theta=c.rope_theta, scale=d ** -0.5,
+                              max_len=self.ctx_max, out=self.attn, workspace=self.attn_ws)
+            return
+        ops.gqa_decode(q, k, v, self.k_cache[li], self.v_cache[li], self.pos, n_q_heads=c.n_heads,
+                       n_kv_heads=c.n_kv_heads, theta=c.rope_theta, scale=d ** -0.5, max_len=self.ctx_max,
+                       out=self.attn, workspace=self.attn_ws, prefetch_kv=prefetch)
+
     def _step_gemm(self) -> torch.Tensor:
         """Large-batch step: tcgen05 GEMMs for every projection (packed weights, A in TMEM),
         RMSNorm fused into their x pre-pass."""
         c = self.cfg
-        d = c.head_dim
-        qd, kd = c.n_heads * d, c.n_kv_heads * d
         ws = self.gemm_ws
         pk = self.packed
         for li, L in enumerate(self.w["layers"]):
@@ -197,10 +219,7 @@ class Q4Decoder:
             # RMSNorm fused into the GEMMs' x pre-pass; weights stream before each PDL wait
             ops.q4_gemm(G["qkv"], self.nt_qkv, self.kt_h, self.resid, out=self.qkv, workspace=ws, prefetch=True,
                         norm_w=L["attn_norm"], eps=c.rms_eps, packed=pk)
-            ops.gqa_decode(self.qkv[:, :qd], self.qkv[:, qd:qd + kd], self.qkv[:, qd + kd:],
-                           self.k_cache[li], self.v_cache[li], self.pos, n_q_heads=c.n_heads,
-                           n_kv_heads=c.n_kv_heads, theta=c.rope_theta, scale=d ** -0.5, max_len=self.ctx_max,
-                           out=self.attn, workspace=self.attn_ws, prefetch_kv=True)
+            self._attend(li, True)
             ops.q4_gemm(G["o"], self.nt_h, self.kt_q, self.attn, out=self.resid, accumulate=True, workspace=ws,
                         prefetch=True, packed=pk)
             ops.q4_swiglu_gemm(G["gate"], G["up"], self.nt_i, self.kt_h, self.resid, out=self.h, workspace=ws,
@@ -236,7 +255,9 @@ class Q4Decoder:
     def bytes_per_step(self, lengths) -> int:
         """Algorithmic HBM bytes of one step: weights + KV read (+ new token written)."""
         wb = self.cfg.weight_bytes()
-        kv = sum(int(n) for n in lengths) * self.cfg.n_kv_heads * self.cfg.head_dim * 2 * 2 * self.cfg.n_layers
+        row = (self.cache.bytes_per_token() if self.cache is not None
+               else self.cfg.n_kv_heads * self.cfg.head_dim * 2 * 2)
+        kv = sum(int(n) for n in lengths) * row * self.cfg.n_layers
         return wb["layers"] + wb["lm_head"] + kv
 
 

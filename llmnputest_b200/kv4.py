@@ -1,0 +1,111 @@
+"""A 4-bit paged KV cache for batched decode: the pages of every layer, and which row holds which.
+
+`ops.kv4_*` are the operators; this keeps their buffers together for a server or a decoder:
+
+    cache = Kv4Cache(n_layers, n_pages, n_kv_heads, head_dim, batch, max_pages)
+    cache.reserve(prompt_lens)                       # pages for every row's next tokens
+    for l in range(n_layers): cache.append(l, k, v, pos, cu=cu)       # prompts, ragged
+    cache.advance(prompt_lens)
+    ...
+    cache.reserve(1)                                 # a decode step: one more token a row
+    for l in ...: cache.append(l, k, v, pos); out = cache.decode(l, q, pos, n_q_heads=40)
+    cache.advance(1)
+    cache.reorder(parent)                            # beams, new requests, rows that ended
+
+A value takes 4.5 bits (codes of 4 bits, a bf16 step and least value per token, kv head and
+64 dims) where the dense cache of `ops.gqa_decode` takes 16.  Rows share full pages; the table
+and its counts live on the device and nothing here waits for it: `info` of the last reorder or
+compact can be read when a host wants to know what is free.  The buffers stay where they are,
+so a captured step sees what later calls put into them.  No reference counterpart (the reference
+keeps one sequence's K and V in bf16, designs/granite_gemv/granite_attention.h:80-213)."""
+
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+
+class Kv4Cache:
+    """Pages, page table, lengths and page counts; see the module's text for a run of calls."""
+
+    def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, batch: int, max_pages: int,
+                 page: int = 64, device=None, summaries: bool = False):
+        """page: tokens of a page, a multiple of 16.  summaries: keep the least and the largest
+        key of every page per dim (4 bytes a kv head and dim), for decode's n_sel."""
+        if min(n_layers, n_pages, n_kv_heads, batch, max_pages) < 1:
+            raise ValueError("every size of a cache is 1 or more")
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.page, self.head_dim, self.n_kv_heads, self.batch, self.max_pages = (page, head_dim, n_kv_heads, batch,
+                                                                                 max_pages)
+        nbytes = ops.kv4_page_bytes(page, head_dim)
+        self.pool = torch.zeros(n_layers, n_pages, n_kv_heads, nbytes, dtype=torch.uint8, device=dev)
+        self.summary = (torch.zeros(n_layers, n_pages, n_kv_heads, 2, head_dim, dtype=torch.bfloat16, device=dev)
+                        if summaries else None)
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.table = torch.full((batch, max_pages), -1, **i32)
+        self.lens = torch.zeros(batch, **i32)
+        self.refs = torch.zeros(n_pages, **i32)
+        self.info = torch.zeros(4, **i32)
+        self._same = torch.arange(batch, **i32)
+        self._layers = list(self.pool.unbind(0))
+        self._near = list(self.summary.unbind(0)) if summaries else [None] * n_layers
+
+    def bytes_per_token(self) -> int:
+        """Bytes of one token's K and V in one layer."""
+        return self.n_kv_heads * self.head_dim * 9 // 8
+
+    def reorder(self, parent: torch.Tensor, reserve: torch.Tensor | None = None) -> torch.Tensor:
+        """Row b goes on with the tokens of row parent[b] (-1: with none), and has pages for
+        reserve[b] more (ops.kv4_reorder).  Returns info: free pages left, pages copied, pages
+        missing, 0."""
+        table, lens, refs, info = ops.kv4_reorder(self.pool, self.table, self.lens, self.refs, parent,
+                                                  head_dim=self.head_dim, reserve=reserve, summary=self.summary)
+        self.table.copy_(table)
+        self.lens.copy_(lens)
+        self.refs.copy_(refs)
+        self.info.copy_(info)
+        return self.info
+
+    def reserve(self, tokens: int | torch.Tensor) -> torch.Tensor:
+        """Pages for that many tokens behind those that every row has (int32 [batch], or one number)."""
+        if not isinstance(tokens, torch.Tensor):
+            tokens = torch.full_like(self.lens, int(tokens))
+        return self.reorder(self._same, tokens)
+
+    def compact(self) -> torch.Tensor:
+        """Live pages to the lowest numbers (ops.kv4_compact).  Returns info: live pages, pages moved, 0, 0."""
+        table, refs, info = ops.kv4_compact(self.pool, self.table, self.refs, summary=self.summary)
+        self.table.copy_(table)
+        self.refs.copy_(refs)
+        self.info.copy_(info)
+        return self.info
+
+    def advance(self, tokens: int | torch.Tensor) -> None:
+        """The rows have that many more tokens (what has been appended to every layer)."""
+        self.lens.add_(tokens)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, *,
+               cu: torch.Tensor | None = None, theta: float | None = 10000.0) -> None:
+        """New rows of one layer at positions pos (ops.kv4_append)."""
+        ops.kv4_append(k, v, self._layers[layer], self.table, pos, n_kv_heads=self.n_kv_heads,
+                       head_dim=self.head_dim, cu=cu, theta=theta, summary=self._near[layer])
+
+    def gather(self, layer: int, pos: torch.Tensor, rows: int, *, cu: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows of one layer read back (ops.kv4_gather)."""
+        return ops.kv4_gather(self._layers[layer], self.table, pos, rows, n_kv_heads=self.n_kv_heads,
+                              head_dim=self.head_dim, cu=cu, dtype=dtype)
+
+    def decode(self, layer: int, q: torch.Tensor, pos: torch.Tensor, *, n_q_heads: int, theta: float | None = 10000.0,
+               scale: float | None = None, n_sel: int | None = None, **kw) -> torch.Tensor:
+        """Attention of one query per row over tokens 0..pos (ops.kv4_decode), or over the n_sel
+        pages that ops.kv4_select picks for it (a cache with summaries)."""
+        heads = dict(n_q_heads=n_q_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, theta=theta)
+        select = None
+        if n_sel is not None:
+            if self.summary is None:
+                raise ValueError("n_sel needs a cache with summaries")
+            select = ops.kv4_select(q, self._near[layer], self.table, pos, page=self.page,
+                                    n_sel=min(n_sel, self.max_pages), **heads)
+        return ops.kv4_decode(q, self._layers[layer], self.table, pos, scale=scale, select=select, **heads, **kw)

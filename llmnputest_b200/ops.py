@@ -635,7 +635,8 @@ def _kv4_need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.devi
 def _kv4_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, rows: int, width: int) -> int:
     """The row stride of [rows, >= width] with unit column stride."""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.dim() == 2:
-        (n, w), (ld, unit) = t.shape, t.stride()
+        n, w = t.shape
+        ld, unit = t.stride()
         if n == rows and w >= width and (unit == 1 or w == 1):
             return ld if n > 1 else w
     _need(t, name, dtype)
@@ -644,29 +645,35 @@ def _kv4_rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.devi
     raise ValueError(f"{name} must be [{rows}, >= {width}] with unit column stride, got {tuple(t.shape)}")
 
 
-def _kv4_table(table: torch.Tensor, device: torch.device) -> torch.Size:
-    """[batch, max_pages] of a page table."""
+def _kv4_table(table: torch.Tensor, pos: torch.Tensor, what: str, device: torch.device) -> tuple[int, int, int, int]:
+    """[batch, max_pages] of a page table, its address and that of `pos` [batch]."""
+    if (isinstance(table, torch.Tensor) and table.dtype is torch.int32 and table.dim() == 2 and table.device == device
+            and table.is_contiguous()):
+        batch, max_pages = table.shape
+        if batch and max_pages:
+            return batch, max_pages, table.data_ptr(), _kv4_need(pos, what, torch.int32, device, (batch,))
     _kv4_need(table, "table", torch.int32, device)
-    if table.dim() != 2 or not table.numel():
-        raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
-    return table.shape
+    raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
 
 
-def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> tuple[int, int]:
-    """(pages, page length) of one layer's pool."""
+def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> tuple[int, int, torch.device]:
+    """(pages, page length, device) of one layer's pool."""
+    if isinstance(pool, torch.Tensor) and pool.dtype is torch.uint8 and pool.dim() == 3 and pool.is_contiguous():
+        n_pages, hkv, nbytes = pool.shape
+        device = pool.device
+        if hkv == n_kv_heads and device.type == "cuda":
+            return n_pages, _kv4_page(nbytes, head_dim), device
     _need(pool, "pool", torch.uint8)
-    if pool.dim() != 3 or pool.shape[1] != n_kv_heads or not pool.is_contiguous():
-        raise ValueError(f"pool must be contiguous [n_pages, {n_kv_heads}, page bytes], got {tuple(pool.shape)}")
-    return pool.shape[0], _kv4_page(pool.shape[2], head_dim)
+    raise ValueError(f"pool must be contiguous [n_pages, {n_kv_heads}, page bytes], got {tuple(pool.shape)}")
 
 
 def _kv4_call(device: torch.device, name: str, *args) -> None:
     """A call on `device`'s current stream, whichever device is current."""
     index = device.index
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(device):
             return _kv4_call(device, name, *args)
-    status = getattr(_native.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    status = getattr(_native._LIB or _native.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _native.check(status, name)
 
@@ -679,12 +686,12 @@ def _kv4_ws_bytes(device: int, name: str, *args) -> int:
     return n.value
 
 
-def _kv4_ws(workspace: torch.Tensor | None, need: int, device: torch.device) -> torch.Tensor | None:
-    if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if _kv4_need(workspace, "workspace", torch.uint8, device) % 16 or workspace.numel() < need:
+def _kv4_ws_at(workspace: torch.Tensor, need: int, device: torch.device) -> tuple[int, int]:
+    """Address and size of a workspace that the caller keeps."""
+    at = _kv4_need(workspace, "workspace", torch.uint8, device)
+    if at % 16 or workspace.numel() < need:
         raise ValueError(f"workspace must hold {need} bytes, 16-byte aligned")
-    return workspace
+    return at, workspace.numel()
 
 
 def _kv4_cu(cu: torch.Tensor | None, batch: int, rows: int, device: torch.device) -> int | None:
@@ -705,20 +712,19 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torc
     int32 [B], the position of each sequence's first new row (-1: none); cu int32 [B + 1]
     row offsets (None: one row per sequence); theta None: keys are stored as given; summary
     bf16 [n_pages, Hkv, 2, D] takes the new keys in (for kv4_select)."""
-    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
-    dev, dtype, rows = pool.device, k.dtype, k.shape[0]
-    batch, max_pages = _kv4_table(table, dev)
+    n_pages, page, dev = _kv4_pool(pool, n_kv_heads, head_dim)
+    batch, max_pages, pages, at = _kv4_table(table, pos, "pos", dev)
+    dtype, rows = k.dtype, k.shape[0]
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("k must be fp32 or bf16")
     ld_k = _kv4_rows(k, "k", dtype, dev, rows, n_kv_heads * head_dim)
     ld_v = _kv4_rows(v, "v", dtype, dev, rows, n_kv_heads * head_dim)
-    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     offsets = _kv4_cu(cu, batch, rows, dev)
     near = (None if summary is None else
             _kv4_need(summary, "summary", torch.bfloat16, dev, (n_pages, n_kv_heads, 2, head_dim)))
     flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_ROWS_F32 if dtype is torch.float32 else 0)
-    _kv4_call(dev, "b2_kv4_append", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), table.data_ptr(),
-              at, offsets, near, batch, n_kv_heads, head_dim, page, max_pages, n_pages, theta or 0.0, flags)
+    _kv4_call(dev, "b2_kv4_append", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), pages, at, offsets,
+              near, batch, n_kv_heads, head_dim, page, max_pages, n_pages, theta or 0.0, flags)
 
 
 def kv4_gather(pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, rows: int, *, n_kv_heads: int,
@@ -729,18 +735,22 @@ def kv4_gather(pool: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, rows:
     Sequence b's tokens pos[b], pos[b] + 1, ... go to rows cu[b] .. cu[b+1] - 1 (cu None:
     one token per sequence).  dtype bf16 or fp32.  Rows that no token goes to keep what
     `out` holds; without `out` they are not set."""
-    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
-    dev, width = pool.device, n_kv_heads * head_dim
-    batch, max_pages = _kv4_table(table, dev)
+    n_pages, page, dev = _kv4_pool(pool, n_kv_heads, head_dim)
+    batch, max_pages, pages, at = _kv4_table(table, pos, "pos", dev)
+    width = n_kv_heads * head_dim
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("dtype must be fp32 or bf16")
-    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     offsets = _kv4_cu(cu, batch, rows, dev)
-    k, v = out if out is not None else torch.empty((2, rows, width), dtype=dtype, device=dev).unbind(0)
-    ld_k = _kv4_rows(k, "out k", dtype, dev, rows, width)
-    ld_v = _kv4_rows(v, "out v", dtype, dev, rows, width)
-    _kv4_call(dev, "b2_kv4_gather", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), table.data_ptr(), at,
-              offsets, batch, n_kv_heads, head_dim, page, max_pages, n_pages,
+    if out is None:
+        k = torch.empty((rows, width), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        ld_k = ld_v = width
+    else:
+        k, v = out
+        ld_k = _kv4_rows(k, "out k", dtype, dev, rows, width)
+        ld_v = _kv4_rows(v, "out v", dtype, dev, rows, width)
+    _kv4_call(dev, "b2_kv4_gather", k.data_ptr(), v.data_ptr(), ld_k, ld_v, rows, pool.data_ptr(), pages, at, offsets,
+              batch, n_kv_heads, head_dim, page, max_pages, n_pages,
               KV4_ROWS_F32 if dtype is torch.float32 else 0)
     return k, v
 
@@ -763,15 +773,15 @@ def kv4_decode(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: to
     zeros).  select int32 [B, Hkv, n_sel] (kv4_select): attend to those pages alone.
     max_len (default: the table's) bounds pos + 1 and sizes the split.  Returns [B, Hq*D]
     bf16, or fp32 with out_f32."""
-    n_pages, page = _kv4_pool(pool, n_kv_heads, head_dim)
-    dev, width = pool.device, n_q_heads * head_dim
-    batch, max_pages = _kv4_table(table, dev)
+    n_pages, page, dev = _kv4_pool(pool, n_kv_heads, head_dim)
+    batch, max_pages, pages, at = _kv4_table(table, pos, "pos", dev)
+    width = ldo = n_q_heads * head_dim
     ld_q = _kv4_rows(q, "q", torch.float32, dev, batch, width)
-    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     odt = torch.float32 if out_f32 else torch.bfloat16
     if out is None:
-        out = torch.empty((batch, width), dtype=odt, device=dev)
-    ldo = _kv4_rows(out, "out", odt, dev, batch, width)
+        out = q.new_empty((batch, width), dtype=odt)
+    else:
+        ldo = _kv4_rows(out, "out", odt, dev, batch, width)
     chosen, n_sel = None, 0
     if select is not None:
         _need(select, "select", torch.int32)
@@ -783,12 +793,16 @@ def kv4_decode(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, pos: to
         max_len = max_pages * page
     need = _kv4_ws_bytes(dev.index, "b2_kv4_decode_workspace_size", batch, n_q_heads, n_kv_heads, head_dim, page,
                          n_sel, max_len)
-    ws = _kv4_ws(workspace, need, dev)
+    ws, size = None, 0
+    if workspace is not None:
+        ws, size = _kv4_ws_at(workspace, need, dev)
+    elif need:
+        own = pool.new_empty(need)
+        ws, size = own.data_ptr(), need
     flags = (KV4_NO_ROPE if theta is None else 0) | (KV4_OUT_F32 if out_f32 else 0)
-    _kv4_call(dev, "b2_kv4_decode", q.data_ptr(), ld_q, pool.data_ptr(), table.data_ptr(), at, chosen, n_sel, batch,
+    _kv4_call(dev, "b2_kv4_decode", q.data_ptr(), ld_q, pool.data_ptr(), pages, at, chosen, n_sel, batch,
               n_q_heads, n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0,
-              head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
-              None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), flags)
+              head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ldo, ws, size, flags)
     return out
 
 
@@ -804,17 +818,18 @@ def kv4_select(q: torch.Tensor, summary: torch.Tensor, table: torch.Tensor, pos:
     _need(summary, "summary", torch.bfloat16)
     dev, n_pages = summary.device, summary.shape[0]
     near = _kv4_need(summary, "summary", torch.bfloat16, dev, (n_pages, n_kv_heads, 2, head_dim))
-    batch, max_pages = _kv4_table(table, dev)
+    batch, max_pages, pages, at = _kv4_table(table, pos, "pos", dev)
     ld_q = _kv4_rows(q, "q", torch.float32, dev, batch, n_q_heads * head_dim)
-    at = _kv4_need(pos, "pos", torch.int32, dev, (batch,))
     if n_sel < 1:
         raise ValueError("n_sel must be >= 1")
     if out is None:
-        out = torch.empty((batch, n_kv_heads, n_sel), dtype=torch.int32, device=dev)
-    chosen = _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
+        out = table.new_empty((batch, n_kv_heads, n_sel))
+        chosen = out.data_ptr()
+    else:
+        chosen = _kv4_need(out, "out", torch.int32, dev, (batch, n_kv_heads, n_sel))
     if max_len is None:
         max_len = max_pages * page
-    _kv4_call(dev, "b2_kv4_select", q.data_ptr(), ld_q, near, table.data_ptr(), at, chosen, n_sel, batch, n_q_heads,
+    _kv4_call(dev, "b2_kv4_select", q.data_ptr(), ld_q, near, pages, at, chosen, n_sel, batch, n_q_heads,
               n_kv_heads, head_dim, page, max_pages, n_pages, max_len, theta or 0.0, KV4_NO_ROPE if theta is None else 0)
     return out
 
@@ -826,15 +841,14 @@ def _kv4_layers(pool: torch.Tensor, summary: torch.Tensor | None) -> tuple:
     if pool.dim() != 4 or not pool.is_contiguous():
         raise ValueError(f"pool must be contiguous [layers, n_pages, Hkv, page bytes], got {tuple(pool.shape)}")
     layers, n_pages, hkv, nbytes = pool.shape
-    near, near_bytes = None, 0
-    if summary is not None:
-        _need(summary, "summary", torch.bfloat16)
-        if summary.dim() != 5:
-            raise ValueError(f"summary must be [layers, n_pages, Hkv, 2, D], got {tuple(summary.shape)}")
-        dim = summary.shape[4]
-        near = _kv4_need(summary, "summary", torch.bfloat16, pool.device, (layers, n_pages, hkv, 2, dim))
-        near_bytes = 4 * hkv * dim
-    return pool.data_ptr(), hkv * nbytes, near, near_bytes, layers, n_pages
+    if summary is None:
+        return pool.data_ptr(), hkv * nbytes, None, 0, layers, n_pages
+    _need(summary, "summary", torch.bfloat16)
+    if summary.dim() != 5:
+        raise ValueError(f"summary must be [layers, n_pages, Hkv, 2, D], got {tuple(summary.shape)}")
+    dim = summary.shape[4]
+    near = _kv4_need(summary, "summary", torch.bfloat16, pool.device, (layers, n_pages, hkv, 2, dim))
+    return pool.data_ptr(), hkv * nbytes, near, 4 * hkv * dim, layers, n_pages
 
 
 def kv4_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -862,17 +876,19 @@ def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, ref
     reserve int32 [B]; refs int32 [n_pages].  Returns (table, lens, refs, info) anew; info
     int32 [4]: free pages left, pages copied, pages missing, 0."""
     args = _kv4_layers(pool, summary)
-    dev, n_pages, page = pool.device, pool.shape[1], _kv4_page(pool.shape[3], head_dim)
-    batch, max_pages = _kv4_table(table, dev)
-    rows = (_kv4_need(lens, "lens", torch.int32, dev, (batch,)), _kv4_need(refs, "refs", torch.int32, dev, (n_pages,)),
+    dev, n_pages, page = pool.device, args[-1], _kv4_page(pool.shape[3], head_dim)
+    batch, max_pages, pages, length = _kv4_table(table, lens, "lens", dev)
+    rows = (length, _kv4_need(refs, "refs", torch.int32, dev, (n_pages,)),
             _kv4_need(parent, "parent", torch.int32, dev, (batch,)),
             None if reserve is None else _kv4_need(reserve, "reserve", torch.int32, dev, (batch,)))
-    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, n_pages), dev)
-    # the new rows are parts of one allocation
-    info, refs_out, lens_out, table_out = torch.empty(4 + n_pages + batch + batch * max_pages, dtype=torch.int32,
-                                                      device=dev).split([4, n_pages, batch, batch * max_pages])
-    _kv4_call(dev, "b2_kv4_reorder", *args, table.data_ptr(), *rows, batch, max_pages, page, table_out.data_ptr(),
-              lens_out.data_ptr(), refs_out.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel())
+    need = _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, n_pages)
+    # the workspace and the new rows are parts of one allocation
+    extra = (need + 15) // 16 * 4 if workspace is None else 0
+    own, info, refs_out, lens_out, table_out = table.new_empty(extra + 4 + n_pages + batch + batch * max_pages).split(
+        (extra, 4, n_pages, batch, batch * max_pages))
+    ws, size = (own.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
+    _kv4_call(dev, "b2_kv4_reorder", *args, pages, *rows, batch, max_pages, page, table_out.data_ptr(),
+              lens_out.data_ptr(), refs_out.data_ptr(), info.data_ptr(), ws, size)
     return table_out.view(batch, max_pages), lens_out, refs_out, info
 
 
@@ -881,12 +897,17 @@ def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, 
     """A cache's live pages moved to the lowest page numbers (see b2_kv4_compact).  Returns
     (table, refs, info) anew; info int32 [4]: live pages, pages moved, 0, 0."""
     args = _kv4_layers(pool, summary)
-    dev, n_pages = pool.device, pool.shape[1]
-    batch, max_pages = _kv4_table(table, dev)
+    dev, n_pages = pool.device, args[-1]
+    pages = _kv4_need(table, "table", torch.int32, dev)
+    if table.dim() != 2 or not table.numel():
+        raise ValueError(f"table must be [batch, max_pages], got {tuple(table.shape)}")
+    batch, max_pages = table.shape
     held = _kv4_need(refs, "refs", torch.int32, dev, (n_pages,))
-    ws = _kv4_ws(workspace, _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", n_pages), dev)
-    info, refs_out, table_out = torch.empty(4 + n_pages + batch * max_pages, dtype=torch.int32,
-                                            device=dev).split([4, n_pages, batch * max_pages])
-    _kv4_call(dev, "b2_kv4_compact", *args, table.data_ptr(), held, batch, max_pages, table_out.data_ptr(),
-              refs_out.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel())
+    need = _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", n_pages)
+    extra = (need + 15) // 16 * 4 if workspace is None else 0
+    own, info, refs_out, table_out = table.new_empty(extra + 4 + n_pages + batch * max_pages).split(
+        (extra, 4, n_pages, batch * max_pages))
+    ws, size = (own.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
+    _kv4_call(dev, "b2_kv4_compact", *args, pages, held, batch, max_pages, table_out.data_ptr(), refs_out.data_ptr(),
+              info.data_ptr(), ws, size)
     return table_out.view(batch, max_pages), refs_out, info
