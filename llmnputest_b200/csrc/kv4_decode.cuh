@@ -178,6 +178,12 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+__device__ __forceinline__ uint32_t f16x2_max_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // NT tiles of 16 tokens; the G cells of tile n start at tile0 + n * stride.  MASK: only
 // left[n] of its tokens count.
 template <int D, int NT, bool MASK>
@@ -187,7 +193,8 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
   constexpr int G = D / kKv4Group;
   constexpr uint32_t kLo = 0x000F000Fu;
   const int lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
-  float y[NT][4], e[NT][G][2], f[NT][G][2], emax[NT][2];
+  float y[NT][4];
+  uint2 vm[NT][G];  // (e, f) of tokens gl and gl + 8 as they are stored
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
@@ -196,7 +203,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
       const uint8_t* at = tile0 + n * stride + g * kKv4CellBytes;
       const uint4 kw = *reinterpret_cast<const uint4*>(at + gl * 64 + c * 16);
       const uint2 km = *reinterpret_cast<const uint2*>(at + kKv4KMeta + gl * 8);
-      const uint2 vm = *reinterpret_cast<const uint2*>(at + kKv4VMeta + gl * 8);
+      vm[n][g] = *reinterpret_cast<const uint2*>(at + kKv4VMeta + gl * 8);
       float a[4];
       // words kw.x, kw.y are token gl's, kw.z, kw.w token gl + 8's
       const uint32_t t0[2] = {kw.x, kw.y}, t1[2] = {kw.z, kw.w};
@@ -212,67 +219,71 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
       y[n][1] = fmaf(d0, a[1], fmaf(m0, qs[g][1], y[n][1]));
       y[n][2] = fmaf(d1, a[2], fmaf(m1, qs[g][0], y[n][2]));
       y[n][3] = fmaf(d1, a[3], fmaf(m1, qs[g][1], y[n][3]));
-      e[n][g][0] = fmaxf(bf16lo_to_f32(vm.x), kKv4MinStep);
-      f[n][g][0] = bf16hi_to_f32(vm.x);
-      e[n][g][1] = fmaxf(bf16lo_to_f32(vm.y), kKv4MinStep);
-      f[n][g][1] = bf16hi_to_f32(vm.y);
     }
     if (MASK) {  // what lies behind the last token may hold anything
+      constexpr uint32_t kNothing = 0x2B80u;  // e = 2^-40, f = 0
+      if (gl >= left[n]) {
+        y[n][0] = y[n][1] = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (gl + 8 * i >= left[n]) {
-          y[n][2 * i] = y[n][2 * i + 1] = -INFINITY;
+        for (int g = 0; g < G; ++g) vm[n][g].x = kNothing;
+      }
+      if (gl + 8 >= left[n]) {
+        y[n][2] = y[n][3] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            e[n][g][i] = kKv4MinStep;
-            f[n][g][i] = 0.f;
-          }
-        }
-    }
-    emax[n][0] = e[n][0][0];
-    emax[n][1] = e[n][0][1];
-#pragma unroll
-    for (int g = 1; g < G; ++g) {
-      emax[n][0] = fmaxf(emax[n][0], e[n][g][0]);
-      emax[n][1] = fmaxf(emax[n][1], e[n][g][1]);
+        for (int g = 0; g < G; ++g) vm[n][g].y = kNothing;
+      }
     }
   }
-  float pr[NT][4], top = 0.f;
+  float pr[NT][4];
+  uint32_t w[NT][G][2];  // the weights of heads 2c, 2c + 1, for token gl and token gl + 8
+  // weights against the present R; whether one of them has come to 2^10, or is not a number
+  auto weigh = [&]() -> bool {
+    uint32_t top = 0;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pr[n][i] = kv4_ex2(fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
-    top = fmaxf(top, fmaxf(fmaxf(pr[n][0], pr[n][1]) * emax[n][0], fmaxf(pr[n][2], pr[n][3]) * emax[n][1]));
-  }
-  if (__any_sync(0xffffffffu, top > 1024.f)) {
+      for (int i = 0; i < 4; ++i) pr[n][i] = kv4_ex2(fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float e0 = bf16lo_to_f32(vm[n][g].x), e1 = bf16lo_to_f32(vm[n][g].y);
+        w[n][g][0] = pack_f16x2(pr[n][0] * e0, pr[n][1] * e0);
+        w[n][g][1] = pack_f16x2(pr[n][2] * e1, pr[n][3] * e1);
+        top = f16x2_max_nan(top, f16x2_max_nan(w[n][g][0], w[n][g][1]));
+      }
+    }
+    return (top + 0x1C001C00u) & 0x80008000u;  // 0x6400 is 2^10
+  };
+  if (__any_sync(0xffffffffu, weigh())) {
     // raise R to the largest s + log2 e seen, and rescale what has been summed against the old one
     float r[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i & 1] = fmaxf(r[i & 1], fmaf(y[n][i], unit[i & 1], log2f(emax[n][i >> 1])));
+      for (int i = 0; i < 4; ++i) {
+        float e = kKv4MinStep;
+#pragma unroll
+        for (int g = 0; g < G; ++g) e = fmaxf(e, bf16lo_to_f32(i < 2 ? vm[n][g].x : vm[n][g].y));
+        r[i & 1] = fmaxf(r[i & 1], fmaf(y[n][i], unit[i & 1], log2f(e)));
+      }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) r[i] = fmaxf(r[i], __shfl_xor_sync(0xffffffffu, r[i], o));
       r[i] = fmaxf(r[i], st.r[i]);
-      const float s = kv4_ex2(st.r[i] - r[i]);
+      const float f = kv4_ex2(st.r[i] - r[i]);
       st.r[i] = r[i];
-      st.l[i] *= s;
+      st.l[i] *= f;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        st.m[g][i] *= s;
+        st.m[g][i] *= f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          st.o[g][k][i] *= s;
-          st.o[g][k][i + 2] *= s;
+          st.o[g][k][i] *= f;
+          st.o[g][k][i + 2] *= f;
         }
       }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pr[n][i] = kv4_ex2(fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
+    weigh();
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -280,10 +291,10 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
     st.l[1] += pr[n][1] + pr[n][3];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      st.m[g][0] = fmaf(pr[n][0], f[n][g][0], fmaf(pr[n][2], f[n][g][1], st.m[g][0]));
-      st.m[g][1] = fmaf(pr[n][1], f[n][g][0], fmaf(pr[n][3], f[n][g][1], st.m[g][1]));
-      const uint32_t b0 = movmatrix_trans(pack_f16x2(pr[n][0] * e[n][g][0], pr[n][1] * e[n][g][0]));
-      const uint32_t b1 = movmatrix_trans(pack_f16x2(pr[n][2] * e[n][g][1], pr[n][3] * e[n][g][1]));
+      const float f0 = bf16hi_to_f32(vm[n][g].x), f1 = bf16hi_to_f32(vm[n][g].y);
+      st.m[g][0] = fmaf(pr[n][0], f0, fmaf(pr[n][2], f1, st.m[g][0]));
+      st.m[g][1] = fmaf(pr[n][1], f0, fmaf(pr[n][3], f1, st.m[g][1]));
+      const uint32_t b0 = movmatrix_trans(w[n][g][0]), b1 = movmatrix_trans(w[n][g][1]);
       const uint4 v = *reinterpret_cast<const uint4*>(tile0 + n * stride + g * kKv4CellBytes + kKv4VCodes + gl * 64 + c * 16);
       float(&o)[4][4] = st.o[g];
 #pragma unroll
@@ -495,6 +506,17 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
   // (kBehind: the tile lies behind the lane below's in memory and in its stage)
   int left_now, left_next = 0;
   const uint8_t *at_now, *at_next;
+  // of the 32 tiles at hand: those with tokens, those full; this lane's copy: the tiles that lie
+  // in a row from its own on, as far as its stage goes
+  unsigned some, full_tiles;
+  int copy_bytes;
+  auto survey = [&]() {
+    some = __ballot_sync(0xffffffffu, left_now > 0);
+    full_tiles = __ballot_sync(0xffffffffu, (left_now & ~kBehind) == kKv4Tile);
+    const unsigned first = __ballot_sync(0xffffffffu, left_now > 0 && !(left_now & kBehind));
+    const int row = __ffs(static_cast<int>(~((some & ~first) >> lane >> 1)));
+    copy_bytes = first >> lane & 1 ? row * Ring::kTileBytes : 0;
+  };
   // the run's first lookups and query on their way (cluster: the query is already)
   auto begin = [&]() {
     run.lg = 0;
@@ -515,29 +537,25 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
     int issued = 0;
     unsigned whole = 0;  // bit s: every tile of the stage in slot s is there and full
     auto issue = [&]() {  // the next stage into slot `in_slot`: the lanes that hold its tiles copy them
-      const int i = issued << run.lg;
-      if ((i & 31) == 0 && i > 0) {
-        at_now = at_next;
-        left_now = left_next;
-        if (i + 32 < run.n_stages << run.lg) at_next = find(i + 32, left_next);
-      }
-      const bool in = (lane >> run.lg) == ((i & 31) >> run.lg);
-      const int left = left_now & ~kBehind;
-      const unsigned some = __ballot_sync(0xffffffffu, in && left > 0);
-      const unsigned all = __ballot_sync(0xffffffffu, in && left == kKv4Tile);
-      // tiles that lie in a row are one copy, by the first one's lane
-      const unsigned first = __ballot_sync(0xffffffffu, in && left_now > 0 && !(left_now & kBehind));
-      const uint32_t bar = bar0 + in_slot * 8, mine = lane & ((1 << run.lg) - 1);
-      whole = (whole & ~(1u << in_slot)) | static_cast<unsigned>(__popc(all) == ST) << in_slot;
-      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(some) * Ring::kTileBytes);
-      __syncwarp();
-      if (in) {
-        left_s[warp][in_slot][mine] = left;
-        if (first >> lane & 1) {
-          // one and the lanes above that go on with it: none outside the stage, as `some` has none there
-          const int row = __ffs(static_cast<int>(~((some & ~first) >> lane >> 1)));
-          bulk_g2s(ring_s + in_slot * Ring::kStageBytes + mine * Ring::kTileBytes, at_now, row * Ring::kTileBytes, bar, once);
+      const int i = issued << run.lg, o = i & 31;
+      if (o == 0) {
+        if (i > 0) {
+          at_now = at_next;
+          left_now = left_next;
+          if (i + 32 < run.n_stages << run.lg) at_next = find(i + 32, left_next);
         }
+        survey();
+      }
+      const unsigned tiles = (1u << (1 << run.lg)) - 1u;
+      const uint32_t bar = bar0 + in_slot * 8, mine = lane - o;
+      const bool all = __popc(full_tiles >> o & tiles) == ST;
+      whole = (whole & ~(1u << in_slot)) | static_cast<unsigned>(all) << in_slot;
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(some >> o & tiles) * Ring::kTileBytes);
+      __syncwarp();
+      if (mine < 1u << run.lg) {
+        if (!all) left_s[warp][in_slot][mine] = left_now & ~kBehind;
+        if (copy_bytes)
+          bulk_g2s(ring_s + in_slot * Ring::kStageBytes + mine * Ring::kTileBytes, at_now, copy_bytes, bar, once);
       }
       in_slot = in_slot + 1 == NS ? 0 : in_slot + 1;
       ++issued;

@@ -195,7 +195,8 @@ static int kv4_decode_check(const Kv4Shape& s, int hq, int n_sel, int max_len) {
   if (st != B2_OK) return st;
   st = kv4_heads(hq, s.hkv);
   if (st != B2_OK) return st;
-  if (n_sel < 0 || n_sel > s.max_pages) return fail(B2_ERR_ARG, "n_sel %d outside 0..max_pages %d", n_sel, s.max_pages);
+  if (n_sel < 0 || static_cast<long long>(n_sel) * s.page > (1LL << 30))
+    return fail(B2_ERR_ARG, "n_sel %d: 0 or more, over 2^30 tokens at most", n_sel);
   if (max_len < 1 || max_len > static_cast<long long>(s.max_pages) * s.page)
     return fail(B2_ERR_ARG, "max_len %d outside 1..max_pages * page", max_len);
   return B2_OK;
@@ -208,7 +209,7 @@ int b2_kv4_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int h
   if (st != B2_OK) return st;
   if (!bytes) return fail(B2_ERR_ARG, "null bytes pointer");
   if (max_len < 1 || page < 1 || n_sel < 0) return fail(B2_ERR_ARG, "bad lengths");
-  st = kv4_decode_check({batch, n_kv_heads, head_dim, page, std::max(n_sel, (max_len - 1) / page + 1), 1}, n_q_heads,
+  st = kv4_decode_check({batch, n_kv_heads, head_dim, page, (max_len - 1) / page + 1, 1}, n_q_heads,
                         n_sel, max_len);
   if (st != B2_OK) return st;
   *bytes = kv4_decode_plan(batch, n_q_heads, n_kv_heads, head_dim, kv4_decode_tokens(n_sel, page, max_len), di.sms).ws_bytes;

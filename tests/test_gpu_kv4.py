@@ -305,9 +305,20 @@ def test_select(ops, dim, page, n_sel, grp):
         got = ops.kv4_select(dev(q), c.summary, c.dtable, c.pos, n_q_heads=hq, page=page, n_sel=n_sel, theta=theta,
                              **c.heads)
         assert np.array_equal(host(got), want)
-    if n_sel <= c.table.shape[1]:
-        got, ref = run_decode(ops, c, grp, rng, select=dev(want), out_f32=True)
-        close(host(got), ref, F32_TOL)
+    got, ref = run_decode(ops, c, grp, rng, select=dev(want), out_f32=True)
+    close(host(got), ref, F32_TOL)
+
+
+@pytest.mark.parametrize("dim,ctx", [(64, 40), (256, 700)])
+def test_more_pages_asked_for_than_there_are(ops, dim, ctx):
+    """n_sel above the pages of the row, and of the whole table: all of them, -1 behind."""
+    rng = np.random.default_rng(ctx)
+    c = Case(rng, [ctx, 3], 2, dim, 16, extra=0)
+    q = rng.standard_normal((2, 4 * dim)).astype(np.float32)
+    sel = ops.kv4_select(dev(q), c.summary, c.dtable, c.pos, n_q_heads=4, page=16, n_sel=64, theta=None, **c.heads)
+    assert np.array_equal(host(sel), c.cache.select(q.reshape(2, 4, dim), c.table, c.lens - 1, 64, None))
+    got, ref = run_decode(ops, c, 2, rng, select=sel, out_f32=True)
+    close(host(got), ref, F32_TOL)
 
 
 def test_select_ties_go_to_the_lower_page(ops):
@@ -606,8 +617,8 @@ def test_refusals(ops):
         (ValueError, lambda: ops.kv4_decode(x, c.pool, c.dtable, c.pos, n_q_heads=18, **ok)),
         (B2Error, lambda: ops.kv4_decode(x, c.pool, c.dtable, c.pos, n_q_heads=4, max_len=10**6, **ok)),
         (ValueError, lambda: ops.kv4_decode(x, c.pool, c.dtable, c.pos, n_q_heads=4, select=c.dtable, **ok)),
-        (B2Error, lambda: ops.kv4_decode(x, c.pool, c.dtable, c.pos, n_q_heads=4,
-                                         select=torch.zeros(2, 2, 50, dtype=torch.int32, device="cuda"), **ok)),
+        (ValueError, lambda: ops.kv4_decode(x, c.pool, c.dtable, c.pos, n_q_heads=4,
+                                            select=torch.zeros(2, 2, 0, dtype=torch.int32, device="cuda"), **ok)),
         (ValueError, lambda: ops.kv4_select(x, c.summary, c.dtable, c.pos, n_q_heads=4, page=16, n_sel=0, **ok)),
         (B2Error, lambda: ops.kv4_select(x, c.summary, c.dtable, c.pos, n_q_heads=4, page=20, n_sel=1, **ok)),
         (ValueError, lambda: ops.kv4_copy_pages(c.pool, c.pos, c.pos)),
