@@ -442,17 +442,29 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
     const int total = sum * p.hkv;  // below 2^30
     const int n_cta = min(total, static_cast<int>(gridDim.x));
     if (static_cast<int>(blockIdx.x) >= n_cta) return;
+    // the share's ends: equal parts of all weights, but a pair's own end where that is within 3%
+    // of a part, so that pairs of nearly one length are not cut in a piece and a crumb
     const int each = total / n_cta, rest = total - each * n_cta, me = blockIdx.x;
-    u = each * me + min(me, rest);
-    u1 = u + each + (me < rest);
-    int b = 0, hi = p.batch;  // the last sequence that begins at or below u, and has tiles
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if (before[mid] * p.hkv <= u) b = mid;
-      else hi = mid;
-    }
+    auto edge = [&](int i, int& b) -> int {
+      const int at = each * i + min(i, rest);
+      b = 0;
+      if (i == n_cta) return total;
+      int hi = p.batch;  // the last sequence that begins at or below `at`, and has tiles
+      while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (before[mid] * p.hkv <= at) b = mid;
+        else hi = mid;
+      }
+      const int weight = before[b + 1] - before[b], in = (at - before[b] * p.hkv) % weight;
+      return in <= each / 32 ? at - in : weight - in <= each / 32 ? at + weight - in : at;
+    };
+    int b;
+    u1 = edge(me + 1, b);
+    u = edge(me, b);
+    if (u >= u1) return;
+    // (an end moved up may be the next sequence's beginning: next() steps on to it)
     run.b = b;
-    run.kvh = (u - before[b] * p.hkv) / (before[b + 1] - before[b]);
+    run.kvh = min((u - before[b] * p.hkv) / (before[b + 1] - before[b]), p.hkv - 1);
   }
   // dealt: the next pair of the share that has tiles in it; false behind the last.  A share may
   // end inside a pair's overhead, which leaves it none of the tiles.

@@ -103,7 +103,16 @@ Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int toke
     pl.splits = s;
     return pl;
   }
-  pl.ctas = static_cast<int>(std::min(slots, (pairs * pl.tiles + 2 * W - 1) / (2 * W)));
+  // a whole number of CTAs a pair, or of pairs a CTA, where that leaves few slots empty: equal
+  // lengths are then not cut (64 sequences x 8 kv heads of 4096 tokens: 512 CTAs of 592)
+  long long n = slots;
+  if (pairs <= slots) {
+    if (slots / pairs * pairs * 10 >= slots * 8) n = slots / pairs * pairs;
+  } else {
+    const long long c = (pairs + slots - 1) / slots;
+    if ((pairs + c - 1) / c * 10 >= slots * 9) n = (pairs + c - 1) / c;
+  }
+  pl.ctas = static_cast<int>(std::min(n, (pairs * pl.tiles + 2 * W - 1) / (2 * W)));
   pl.span_bytes = (static_cast<size_t>(pairs) * 8 + 15) / 16 * 16;
   pl.ws_bytes = pl.span_bytes + static_cast<size_t>(pl.ctas) * 2 * b2::kv4_part_floats(hq / hkv, head_dim) * sizeof(float);
   return pl;
