@@ -10,9 +10,9 @@
 // and as its low nibble a: two byte permutations and two ANDs make four A registers of a word
 // of 8 codes, without a conversion or an offset.  For the scores a q_a + b q_b is
 // (a + 16 b) (q_b / 16) + a (q_a - q_b / 16); of the values' sums, sum w b is
-// (sum w (a + 16 b) - sum w a) / 16 at the end.  The scales multiply the products' fp32 sums.  S^T = K Q^T (16 tokens x 8 heads per
-// instruction), O^T = V^T P^T; P moves from the accumulator's layout to the B operand's
-// with movmatrix.
+// (sum w (a + 16 b) - sum w a) / 16 at the end.  The scales multiply the products' fp32 sums.
+// S^T = K Q^T (16 tokens x 8 heads per instruction), O^T = V^T P^T; P moves from the
+// accumulator's layout to the B operand's with movmatrix.
 //
 // Weights are taken against a running reference R per head (log2 units) instead of the
 // running maximum: w = 2^(s - R) e goes into the product as fp16, R is raised, and the sums
@@ -322,14 +322,23 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
 //   whole ones and the beginning of another, and a second kernel joins the pairs that were
 //   cut.  (One grid row of CTAs per pair left SMs without work at lengths of 1 to 4096, and
 //   every wave of CTAs after the first costs its start and end again.)
-// Inside a CTA the stages of a pair go to the warps in turn; a stage is 4608 bytes, or fewer
-// tiles where warps would be left without one.  Every warp fills a ring of its own with bulk
-// copies, one per tile, a lane each, and looks the pages up 32 tiles at a time.
+// Inside a CTA the stages of a pair go to the warps in turn; a stage is 4608 bytes (two tiles,
+// 9216, at D = 256: 70.4 us against 74.5 at 256 sequences of 2048), or fewer tiles where warps
+// would be left without one.  Every warp fills a ring of its own with bulk copies, one per
+// run of tiles that lie in a row, and looks the pages up 32 tiles at a time.
+//
+// What bounds it: instruction issue and the latency of a tile's chain (products, exponentials,
+// products) with 8 to 16 warps per SM.  64 sequences x 8 kv heads of 4096 tokens (152 MB of
+// cache, 23.2 us at the measured HBM rate) take 37.5 us, 4.0 TB/s; 256 x 2 of 2048 tokens of 256
+// dims (305 MB, 46.5 us) 70.4 us, 4.3 TB/s.  With the arithmetic left out the copies alone take
+// 28 and 60, with the copies left out the arithmetic 35 and 70.  Measured and dropped: stages
+// of half the size (43 us at D = 64), three stages, 5 to 8 CTAs per SM (registers spill), one
+// tile or four at a time, a tile's scores beside the values of the one before.
 template <int D>
 struct Kv4Ring {
   static constexpr int G = D / kKv4Group;
   static constexpr int kTileBytes = G * kKv4CellBytes;
-  static constexpr int kTiles = 4 / G;  // tiles of a stage at most
+  static constexpr int kTiles = D == 256 ? 2 : 4 / G;  // tiles of a stage at most
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kTiles * kTileBytes;
   // what a run costs beside its tiles, in tiles of a CTA (its start and end, about 4 us; 16 at
