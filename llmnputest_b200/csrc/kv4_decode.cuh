@@ -329,9 +329,9 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
 //
 // What bounds it: instruction issue and the latency of a tile's chain (products, exponentials,
 // products) with 8 to 16 warps per SM.  64 sequences x 8 kv heads of 4096 tokens (152 MB of
-// cache, 23.2 us at the measured HBM rate) take 37.5 us, 4.0 TB/s; 256 x 2 of 2048 tokens of 256
-// dims (305 MB, 46.5 us) 70.4 us, 4.3 TB/s.  With the arithmetic left out the copies alone take
-// 28 and 60, with the copies left out the arithmetic 35 and 70.  Measured and dropped: stages
+// cache, 23.2 us at the measured HBM rate) take 37.4 us, 4.1 TB/s; 256 x 2 of 2048 tokens of 256
+// dims (305 MB, 46.5 us) 70.1 us, 4.3 TB/s.  With a tile's arithmetic left out the rest takes
+// 28.5 and 53.8, with the copies left out 34.8 and 66.8.  Measured and dropped: stages
 // of half the size (43 us at D = 64), three stages, 5 to 8 CTAs per SM (registers spill), one
 // tile or four at a time, a tile's scores beside the values of the one before.
 template <int D>
@@ -342,7 +342,7 @@ struct Kv4Ring {
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kTiles * kTileBytes;
   // what a run costs beside its tiles, in tiles of a CTA (its start and end, about 4 us; 16 at
-  // D = 64 measured 1.3 us slower at 16 sequences of 1 to 4096 tokens)
+  // D = 64 measured 1.2 us slower at 16 sequences of 1 to 4096 tokens)
   static constexpr int kOverhead = 32 / G;
 };
 template <int D, int W>
