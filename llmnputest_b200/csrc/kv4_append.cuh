@@ -156,8 +156,8 @@ __device__ __forceinline__ void kv4_load4(const char* src, bool f32, bool wide, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kKv4AppendThreads, D == 64 ? 5 : 5) kv4_append_kernel(const Kv4RowsParams p,
-                                                                         const __grid_constant__ Kv4Rope rope) {
+__global__ void __launch_bounds__(kKv4AppendThreads, 5) kv4_append_kernel(const Kv4RowsParams p,
+                                                                          const __grid_constant__ Kv4Rope rope) {
   constexpr int G = D / kKv4Group, W = kKv4AppendThreads / 32;
   constexpr int LR = D / 8, RW = 32 / LR, STEP = W * RW;  // lanes of a token, tokens of a warp, of the CTA
   // a lane's 8 values are of one group of 64 (D = 64) or of two

@@ -150,6 +150,8 @@ __device__ __forceinline__ void kv4_prepare_query(const Kv4DecodeParams& p, cons
   }
 }
 
+constexpr float kKv4NoScore = -3.402823466e38f;  // R before the first token: below any finite score
+
 // Running state of one warp: heads 2c and 2c + 1 of the lane.
 template <int D>
 struct Kv4State {
@@ -236,13 +238,16 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
   }
   float pr[NT][4];
   uint32_t w[NT][G][2];  // the weights of heads 2c, 2c + 1, for token gl and token gl + 8
-  // weights against the present R; whether one of them has come to 2^10, or is not a number
-  auto weigh = [&]() -> bool {
+  // weights against the present R; whether one of them has come to 2^10, or is not a number.
+  // Against a new R the scores are rounded as they were for it: past 2^27 an unrounded product
+  // may lie further above R than fp16 reaches.
+  auto weigh = [&](bool anew) -> bool {
     uint32_t top = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pr[n][i] = kv4_ex2(fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
+      for (int i = 0; i < 4; ++i)
+        pr[n][i] = kv4_ex2(anew ? __fmul_rn(y[n][i], unit[i & 1]) - st.r[i & 1] : fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float e0 = bf16lo_to_f32(vm[n][g].x), e1 = bf16lo_to_f32(vm[n][g].y);
@@ -253,7 +258,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
     }
     return (top + 0x1C001C00u) & 0x80008000u;  // 0x6400 is 2^10
   };
-  if (__any_sync(0xffffffffu, weigh())) {
+  if (__any_sync(0xffffffffu, weigh(false))) {
     // raise R to the largest s + log2 e seen, and rescale what has been summed against the old one
     float r[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -263,7 +268,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
         float e = kKv4MinStep;
 #pragma unroll
         for (int g = 0; g < G; ++g) e = fmaxf(e, bf16lo_to_f32(i < 2 ? vm[n][g].x : vm[n][g].y));
-        r[i & 1] = fmaxf(r[i & 1], fmaf(y[n][i], unit[i & 1], log2f(e)));
+        r[i & 1] = fmaxf(r[i & 1], __fmul_rn(y[n][i], unit[i & 1]) + log2f(e));
       }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -283,7 +288,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
         }
       }
     }
-    weigh();
+    weigh(true);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -334,6 +339,7 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
 // 28.5 and 53.8, with the copies left out 34.8 and 66.8.  Measured and dropped: stages
 // of half the size (43 us at D = 64), three stages, 5 to 8 CTAs per SM (registers spill), one
 // tile or four at a time, a tile's scores beside the values of the one before.
+constexpr int kKv4RunOverhead = 32;
 template <int D>
 struct Kv4Ring {
   static constexpr int G = D / kKv4Group;
@@ -343,7 +349,7 @@ struct Kv4Ring {
   static constexpr int kStageBytes = kTiles * kTileBytes;
   // what a run costs beside its tiles, in tiles of a CTA (its start and end, about 4 us; 16 at
   // D = 64 measured 1.2 us slower at 16 sequences of 1 to 4096 tokens)
-  static constexpr int kOverhead = 32 / G;
+  static constexpr int kOverhead = kKv4RunOverhead / G;
 };
 template <int D, int W>
 __host__ __device__ constexpr size_t kv4_decode_smem() {
@@ -607,7 +613,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
       for (int i = 0; i < 4; ++i) st.o[g][i][0] = st.o[g][i][1] = st.o[g][i][2] = st.o[g][i][3] = 0.f;
     }
     st.l[0] = st.l[1] = 0.f;
-    st.r[0] = st.r[1] = -1e30f;
+    st.r[0] = st.r[1] = kKv4NoScore;
 
     int done = 0;
     for (; done < run.n_stages; ++done) {
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
     float* part = p.part + (2 * static_cast<size_t>(blockIdx.x) + (t_lo == 0)) * kv4_part_floats(grp, D);
     for (int e = threadIdx.x; e < grp * D; e += W * 32) {
       const int j = e / D, d = e % D;
-      float R = -1e30f, L = 0.f, O = 0.f;
+      float R = kKv4NoScore, L = 0.f, O = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w)
         if (ml[w][j] != 0.f) R = fmaxf(R, mr[w][j]);
@@ -730,7 +736,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
       for (int i = threadIdx.x; i < share; i += W * 32) {
         const int e = split * share + i, j = e / D;
         if (e >= grp * D) break;
-        float R = -1e30f, L = 0.f, O = 0.f;
+        float R = kKv4NoScore, L = 0.f, O = 0.f;
         for (int k = 0; k < p.splits; ++k)
           if (rl[(k * kKv4MaxGroup + j) * 2 + 1] != 0.f) R = fmaxf(R, rl[(k * kKv4MaxGroup + j) * 2]);
         for (int k = 0; k < p.splits; ++k) {
@@ -776,7 +782,7 @@ __global__ void __launch_bounds__(kKv4JoinMost) kv4_join_kernel(const Kv4DecodeP
   const int e = (tid % quads) * V, slice = tid / quads;
   const int at = j0 * D + e, rl = grp * D + j0 + e / D;
   const float* base = p.part + (2 * static_cast<size_t>(max(span.x, 0)) + 1) * step;  // the pair's first part
-  float R = -1e30f, L = 0.f, O[V] = {};
+  float R = kKv4NoScore, L = 0.f, O[V] = {};
   auto add = [&](float r, float l, const float (&o)[V]) {
     if (l == 0.f) return;
     const float m = fmaxf(R, r), f = kv4_ex2(R - m), g = kv4_ex2(r - m);

@@ -245,7 +245,7 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
       kv4_decode_plan(batch, n_q_heads, n_kv_heads, head_dim, kv4_decode_tokens(n_sel, page, max_len), di.sms);
   if (pl.ws_bytes && (!workspace || workspace_bytes < pl.ws_bytes || !aligned(workspace, 16)))
     return fail(B2_ERR_WORKSPACE, "kv4 decode needs %zu bytes of 16-byte aligned workspace", pl.ws_bytes);
-  if ((pl.tiles + 16LL) * n_kv_heads > (1LL << 30)) return fail(B2_ERR_ARG, "a sequence of over 2^34 tokens x kv heads");
+  if ((pl.tiles + static_cast<long long>(b2::kKv4RunOverhead)) * n_kv_heads > (1LL << 30)) return fail(B2_ERR_ARG, "a sequence of over 2^34 tokens x kv heads");
   b2::Kv4DecodeParams p = {};
   p.q = q;
   p.ld_q = ld_q;
@@ -286,7 +286,7 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
       return cudaLaunchKernelEx(&l.cfg, kernel, p, rope);
     }
     // dealt over the grid, a slice of the batch at a time: the weights of a slice fit 32 bits
-    const int slice = static_cast<int>(std::min<long long>(b2::kKv4MaxDealt, (1LL << 30) / ((pl.tiles + 16LL) * n_kv_heads)));
+    const int slice = static_cast<int>(std::min<long long>(b2::kKv4MaxDealt, (1LL << 30) / ((pl.tiles + static_cast<long long>(b2::kKv4RunOverhead)) * n_kv_heads)));
     for (int b0 = 0; b0 < batch; b0 += slice) {
       b2::Kv4DecodeParams part = p;
       part.batch = std::min(slice, batch - b0);

@@ -2,8 +2,9 @@
 //
 //   bound(page) = max over the kv head's q heads of sum_d max(q_d lo_d, q_d hi_d),
 //
-// lo and hi the page's key summary (per dim, over its tokens): no token of the page scores
-// higher with any of the heads.  Per (sequence, kv head) the n_sel pages with the largest
+// lo and hi the page's key summary (per dim, over its tokens): but for the roundings of the
+// summary to bf16 and of the keys to 4 bits no token of the page scores higher with any of
+// the heads.  Per (sequence, kv head) the n_sel pages with the largest
 // bounds are listed, in ascending order of the page; the page of the query's own position
 // is always among them, and of two equal bounds the lower page goes first.
 //

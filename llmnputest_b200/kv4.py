@@ -98,14 +98,17 @@ class Kv4Cache:
                               head_dim=self.head_dim, cu=cu, dtype=dtype)
 
     def decode(self, layer: int, q: torch.Tensor, pos: torch.Tensor, *, n_q_heads: int, theta: float | None = 10000.0,
-               scale: float | None = None, n_sel: int | None = None, **kw) -> torch.Tensor:
+               scale: float | None = None, n_sel: int | None = None, max_len: int | None = None,
+               **kw) -> torch.Tensor:
         """Attention of one query per row over tokens 0..pos (ops.kv4_decode), or over the n_sel
-        pages that ops.kv4_select picks for it (a cache with summaries)."""
+        pages that ops.kv4_select picks for it (a cache with summaries).  max_len, out, out_f32
+        and workspace as ops.kv4_decode takes them."""
         heads = dict(n_q_heads=n_q_heads, n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, theta=theta)
         select = None
         if n_sel is not None:
             if self.summary is None:
                 raise ValueError("n_sel needs a cache with summaries")
             select = ops.kv4_select(q, self._near[layer], self.table, pos, page=self.page,
-                                    n_sel=min(n_sel, self.max_pages), **heads)
-        return ops.kv4_decode(q, self._layers[layer], self.table, pos, scale=scale, select=select, **heads, **kw)
+                                    n_sel=min(n_sel, self.max_pages), max_len=max_len, **heads)
+        return ops.kv4_decode(q, self._layers[layer], self.table, pos, scale=scale, select=select, max_len=max_len,
+                              **heads, **kw)

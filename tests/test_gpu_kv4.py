@@ -632,3 +632,148 @@ def test_refusals(ops):
             call()
             pytest.fail(f"call {i} was not refused")
     assert torch.equal(before, c.pool)
+
+
+# ---------------------------------------------------------------- the ends of the ranges
+
+@pytest.mark.parametrize("scale", [1e9, 1e20, 1e30])
+def test_decode_scores_of_any_size(ops, scale):
+    """Scores far beyond what exp can take, above and below zero: the largest one's value.  One
+    token's key is 2 in every dim, one's -2, the others' below 1 in size, so that no rounding of
+    q (2^-11 of itself) comes near to changing which is largest; beside it the rest is e^-10^8."""
+    rng = np.random.default_rng(3)
+    c = Case(rng, [1, 20, 500, 3], 2, 64, 16, garbage=False)
+    c.cache.meta[:, :, :, :, 0, :, 0] = 2.0 ** -40
+    c.cache.meta[:, :, :, :, 0, :, 1] = kv4.bf16(rng.uniform(-1, 1, c.cache.meta.shape[:4] + (16,)))
+    for b, (hi, lo) in enumerate([(0, 0), (17, 3), (444, 30), (2, 0)]):
+        for t, m in ((lo, -2.0), (hi, 2.0)):
+            c.cache.meta[c.table[b, t // 16], :, 0, :, 0, t % 16, 1] = m
+    c.pool = dev(c.cache.pool())
+    q = 1 + np.abs(rng.standard_normal((4, 4 * 64))).astype(np.float32)
+    for sign in (1, -1):
+        ref = c.cache.decode((sign * q).reshape(4, 4, 64), c.table, c.lens - 1, None, scale).reshape(4, -1)
+        got = ops.kv4_decode(dev(sign * q), c.pool, c.dtable, c.pos, n_q_heads=4, theta=None, scale=scale, out_f32=True,
+                             **c.heads)
+        close(host(got), ref, F32_TOL, f"sign {sign}")
+
+
+def test_decode_of_many_sequences(ops):
+    """More sequences than one launch deals out, some without tokens."""
+    rng = np.random.default_rng(4)
+    lens = rng.integers(0, 40, 2100)
+    lens[[0, 1023, 1024, 2047, 2099]] = [0, 33, 0, 17, 1]
+    c = Case(rng, lens, 2, 64, 16, garbage=False)
+    got, ref = run_decode(ops, c, 1, rng, out_f32=True, theta=None)
+    close(host(got), ref, F32_TOL)
+    assert (host(got)[lens == 0] == 0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_longest_page(ops, dim):
+    """Pages of 4096 tokens: appended across a border, chosen and attended."""
+    rng = np.random.default_rng(dim)
+    start, new = np.array([4000, 0, 4095], np.int32), np.array([200, 3, 1])
+    c = Case(rng, start + new, 1, dim, 4096, garbage=False)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    k, v = (rng.standard_normal((204, dim)).astype(np.float32) for _ in range(2))
+    c.cache.append(k, v, c.table, start, cu, 10000.0)
+    ops.kv4_append(dev(k), dev(v), c.pool, c.dtable, dev(start), cu=dev(cu), summary=c.summary, **c.heads)
+    assert np.array_equal(host(c.pool), c.cache.pool())
+    assert np.array_equal(host(c.summary), c.cache.summary)
+    got, ref = run_decode(ops, c, 4, rng, out_f32=True)
+    close(host(got), ref, F32_TOL)
+    got, ref = run_decode(ops, c, 4, rng, out_f32=True, select=dev(np.array([[[0]], [[0]], [[0]]], np.int32)))
+    close(host(got), ref, F32_TOL)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_append_rows_of_any_alignment(ops, dtype):
+    """Rows that begin at an odd element and follow one another at an odd distance."""
+    rng = np.random.default_rng(6)
+    start, new = np.array([3, 0], np.int32), np.array([30, 9])
+    c = Case(rng, start + new, 2, 64, 16)
+    cu = np.array([0, 30, 39], np.int32)
+    kv = dev(rng.standard_normal((39, 2 * 128 + 3)), dtype)
+    k, v = kv[:, 1:129], kv[:, 130:258]
+    c.cache.append(host(k), host(v), c.table, start, cu, 10000.0)
+    ops.kv4_append(k, v, c.pool, c.dtable, dev(start), cu=dev(cu), summary=c.summary, **c.heads)
+    assert np.array_equal(host(c.pool), c.cache.pool())
+    assert np.array_equal(host(c.summary), c.cache.summary)
+
+
+def test_append_offsets_outside_the_rows(ops):
+    """Row offsets that fall, or lie outside the rows, are kept inside them: nothing is read
+    or written beyond, and the sequences beside them have their tokens."""
+    rng = np.random.default_rng(11)
+    c = Case(rng, [20, 20, 20, 20], 2, 64, 16)
+    k, v = (rng.standard_normal((10, 128)).astype(np.float32) for _ in range(2))
+    cu = np.array([-5, 4, 2, 6, 900], np.int32)  # 0..4, none, 2..6, 6..10
+    start = np.array([1, 2, 3, 4], np.int32)
+    for b, (lo, hi) in enumerate([(0, 4), (0, 0), (2, 6), (6, 10)]):
+        c.cache.append(k[lo:hi], v[lo:hi], c.table[b:b + 1], start[b:b + 1], np.array([0, hi - lo]), 10000.0)
+    ops.kv4_append(dev(k), dev(v), c.pool, c.dtable, dev(start), cu=dev(cu), summary=c.summary, **c.heads)
+    assert np.array_equal(host(c.pool), c.cache.pool())
+    assert np.array_equal(host(c.summary), c.cache.summary)
+
+
+@pytest.mark.parametrize("dim,pages,n_sel", [(64, 16384, 200), (256, 16384, 16383), (128, 4097, 1000)])
+def test_select_among_the_most_pages(ops, dim, pages, n_sel):
+    rng = np.random.default_rng(pages + n_sel)
+    summary = np.sort(rng.standard_normal((pages, 1, 2, dim)), 2)
+    cache = kv4.Cache(1, 1, dim, 16)
+    cache.summary = kv4.bf16(summary)
+    table = rng.permutation(pages).astype(np.int32)[None]
+    q = rng.standard_normal((1, 3 * dim)).astype(np.float32)
+    for pos in (16 * pages - 1, 16 * pages - 17):
+        want = cache.select(q.reshape(1, 3, dim), table, np.array([pos]), n_sel, None)
+        got = ops.kv4_select(dev(q), dev(cache.summary, torch.bfloat16), dev(table), dev(np.array([pos], np.int32)),
+                             n_q_heads=3, n_kv_heads=1, head_dim=dim, page=16, n_sel=n_sel, theta=None)
+        assert np.array_equal(host(got), want)
+
+
+def test_a_pool_past_four_gigabytes(ops):
+    """The same pages at the far end of a pool whose offsets pass 2^32 bytes: appended, gathered,
+    attended, copied by a fork and moved down by a compaction as at its beginning."""
+    rng = np.random.default_rng(12)
+    c = Case(rng, [200, 65], 8, 64, 64, garbage=False)
+    n = c.cache.code.shape[0]
+    page_bytes = c.pool.shape[1] * c.pool.shape[2]
+    total = (1 << 32) // page_bytes + 3 * n
+    far = total - n - 1  # a free page behind them
+    pool = torch.empty(total, 8, c.pool.shape[2], dtype=torch.uint8, device="cuda")
+    pool[far:far + n] = c.pool
+    table = np.where(c.table >= 0, c.table + far, -1).astype(np.int32)
+    k, v = (rng.standard_normal((2, 512)).astype(np.float32) for _ in range(2))
+    at = np.array([199, 64], np.int32)
+    c.cache.append(k, v, c.table, at, None, 10000.0)
+    ops.kv4_append(dev(k), dev(v), pool, dev(table), dev(at), **c.heads)
+    assert np.array_equal(host(pool[far:far + n]), c.cache.pool())
+    got = ops.kv4_gather(pool, dev(table), dev(at), 2, dtype=torch.float32, **c.heads)
+    for i in range(2):
+        want = c.cache.gather(c.table[i], int(at[i]), 1)
+        for a, w in zip(got, want):
+            assert np.array_equal(host(a[i]), w[0].astype(np.float32).astype(np.float64))
+    q = dev(rng.standard_normal((2, 8 * 64)))
+    ref = c.cache.decode(host(q).reshape(2, 8, 64), c.table, at, 10000.0).reshape(2, -1)
+
+    def attend(p, t, rows):
+        got = ops.kv4_decode(q, p, t, dev(at[rows]), n_q_heads=8, out_f32=True, **c.heads)
+        close(host(got), ref[rows], F32_TOL)
+
+    attend(pool, dev(table), [0, 1])
+    refs = torch.ones(total, dtype=torch.int32, device="cuda")  # every page below is held elsewhere
+    refs[far:] = 0
+    live = table[table >= 0]
+    refs[dev(live.astype(np.int64))] = 1
+    # both rows go on with row 0: its last page is copied to a far free page
+    t2, lens, refs2, info = ops.kv4_reorder(pool[None], dev(table), dev((at + 1).astype(np.int32)), refs,
+                                            dev(np.array([0, 0], np.int32)), head_dim=64)
+    assert host(info)[1] == 1 and host(info)[2] == 0 and host(t2)[1, 3] >= far
+    q[1] = q[0]
+    attend(pool, t2, [0, 0])
+    # only these rows' pages are held: they move down to the beginning
+    held = torch.zeros_like(refs2)
+    held[far:] = refs2[far:]
+    t3, refs3, info = ops.kv4_compact(pool[None], t2, held)
+    assert host(t3).max() < host(info)[0] == int((held > 0).sum())
+    attend(pool, t3, [0, 0])
