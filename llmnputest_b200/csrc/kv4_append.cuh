@@ -17,8 +17,13 @@
 // One CTA per (page of a sequence, kv head), so that the page's summary needs no second pass.
 // D / 8 lanes have a token, each two quads of dims (4 l and D / 2 + 4 l: the pairs that turn
 // together), so that what is done once per 64 values is done for 32 / (D / 8) tokens at a
-// time; a warp per token measured 282 instructions a token and head of 64 dims and 26 us for
-// 8192 tokens of 8 heads.  The codes are put together in shared memory as the cell's bytes.
+// time: 182 instructions a token and head of 64 dims, where a warp per token executed 282.  The
+// codes are put together in shared memory as the cell's bytes.
+//
+// What bounds it: those instructions (2 x 64 values turned, compared and divided), at five CTAs
+// per SM.  8192 tokens of 8 heads of 64 appended to 64 sequences and 8192 read back take 29.5 us,
+// 9.2 by the bytes; one token for each of 64 sequences 8.8 us, two launches and their chains of
+// loads.  Six and eight CTAs per SM (fewer registers) measured no less.
 #pragma once
 
 #include "kv4_cell.cuh"

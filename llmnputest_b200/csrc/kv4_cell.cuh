@@ -47,7 +47,7 @@ __device__ __forceinline__ double kv4_turn(const Kv4Rope& rope, int i) {
 
 // cos and sin of u turns in fp64: to the nearest quarter turn, then the Taylor series of an
 // angle of pi/4 at most (the first term left out is below 3e-18).  Without branches, so that
-// several angles are evaluated side by side: a library sincospi each measured 0.7 us an angle.
+// several angles are evaluated side by side.
 __device__ __forceinline__ void kv4_cos_sin(double u, double& cs, double& sn) {
   const double quarter = rint(4.0 * u);
   const double x = fma(quarter, -0.25, u) * 6.283185307179586476925287, y = x * x;

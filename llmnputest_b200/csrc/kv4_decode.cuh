@@ -347,8 +347,8 @@ struct Kv4Ring {
   static constexpr int kTiles = D == 256 ? 2 : 4 / G;  // tiles of a stage at most
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kTiles * kTileBytes;
-  // what a run costs beside its tiles, in tiles of a CTA (its start and end, about 4 us; 16 at
-  // D = 64 measured 1.2 us slower at 16 sequences of 1 to 4096 tokens)
+  // what a run costs beside its tiles, its start and end, in tiles of a CTA (16 at D = 64
+  // measured 1.2 us slower at 16 sequences of 1 to 4096 tokens)
   static constexpr int kOverhead = kKv4RunOverhead / G;
 };
 template <int D, int W>
@@ -762,14 +762,14 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
 }
 
 // Joins the pairs that several CTAs share, and clears the rows of sequences without tokens:
-// grid (kv head, sequence, share of the heads).  A thread joins D / 64 outputs of one head (at 40
-// heads of 64 one each measured 2.3 us less than four, at 8 of 256 four 3 us less than one);
-// threads beyond the outputs take every further part of them (few pairs, many parts each).
+// grid (kv head, sequence, share of the heads).  A thread joins four outputs of one head (one
+// each, at D = 64: 20.7 us against 15.0 for one sequence of 32768); threads beyond the outputs
+// take every further part of them (many parts a pair).
 // The parts' loads set out together: the kernel is two trips to L2 long.
 constexpr int kKv4JoinMost = 512;
 template <int D>
 __global__ void __launch_bounds__(kKv4JoinMost) kv4_join_kernel(const Kv4DecodeParams p) {
-  constexpr int V = D / 64;
+  constexpr int V = 4;
   __shared__ float sh[2 + V][kKv4JoinMost];
   const int kvh = blockIdx.x, b = blockIdx.y, grp = p.hq / p.hkv, tid = threadIdx.x;
   const int heads = grp / gridDim.z, j0 = blockIdx.z * heads, quads = heads * D / V;

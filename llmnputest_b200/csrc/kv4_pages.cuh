@@ -59,8 +59,9 @@ struct Kv4ReorderParams {
 constexpr int kKv4ScanThreads = 1024;
 constexpr int kKv4PlanThreads = 512, kKv4PlanCtas = 8;
 
-// The new rows' entries and counts, and the lowest free pages in order, by one cluster (as one
-// grid after another, three launches and two copies, it took 13 us of the host's time):
+// The new rows' entries and counts, and the lowest free pages in order, by one cluster (one
+// grid after another would be three launches and two copies, and the host's time for those is
+// what bounds a reorder):
 //   the counts copied; a warp per row takes the old row's holds back, the new one's up and
 //   counts what it lacks; every CTA counts the free pages of its share of the pool; then lists
 //   as many of them, from the lowest on, as all rows lack.

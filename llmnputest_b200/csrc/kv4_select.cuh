@@ -13,8 +13,8 @@
 // are further apart than 2 E the choice is the exact one.  Where not (about one kv head in 300
 // of random keys; always with equal bounds), the pages within 2 E of the border are summed again in
 // fp64, with q turned in fp64 and the summaries bf16, every product exact, and chosen by that.
-// (In fp64 throughout the bounds of 512 pages of 8 kv heads took 4.6 us of 9.8, and those of
-// 16 sequences of up to 1024 pages 35 of 45.)
+// (In fp64 throughout 512 pages of 8 kv heads took 9.8 us, and 16 sequences of up to 1024 pages
+// 45 us; so 8.0 and 24.8.)
 //
 // A cluster per (sequence, kv head): its CTAs take every further group of pages, a warp
 // 256 / D pages at a time (D / 8 lanes a page, 8 dims each), and push the bounds into the first

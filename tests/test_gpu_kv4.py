@@ -777,3 +777,13 @@ def test_a_pool_past_four_gigabytes(ops):
     t3, refs3, info = ops.kv4_compact(pool[None], t2, held)
     assert host(t3).max() < host(info)[0] == int((held > 0).sum())
     attend(pool, t3, [0, 0])
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_decode_of_one_far_longer_sequence(ops, dim):
+    """A pair shared by hundreds of CTAs, its parts joined by several threads an output."""
+    rng = np.random.default_rng(dim + 1)
+    c = Case(rng, [20000, 5, 0, 17], 2, dim, 64, garbage=False)
+    for grp in (1, 8):
+        got, ref = run_decode(ops, c, grp, rng, out_f32=True)
+        close(host(got), ref, F32_TOL)
