@@ -21,7 +21,7 @@
 // codes are put together in shared memory as the cell's bytes.
 //
 // What bounds it: those instructions (2 x 64 values turned, compared and divided), at five CTAs
-// per SM.  8192 tokens of 8 heads of 64 appended to 64 sequences and 8192 read back take 29.5 us,
+// per SM.  8192 tokens of 8 heads of 64 in four prompts, appended and read back, take 29.5 us,
 // 9.2 by the bytes; one token for each of 64 sequences 8.8 us, two launches and their chains of
 // loads.  Six and eight CTAs per SM (fewer registers) measured no less.
 #pragma once

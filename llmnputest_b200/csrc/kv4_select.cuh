@@ -14,7 +14,7 @@
 // of random keys; always with equal bounds), the pages within 2 E of the border are summed again in
 // fp64, with q turned in fp64 and the summaries bf16, every product exact, and chosen by that.
 // (In fp64 throughout 512 pages of 8 kv heads took 9.8 us, and 16 sequences of up to 1024 pages
-// 45 us; so 8.0 and 24.8.)
+// 45 us; so 7.7 and 22.7.)
 //
 // A cluster per (sequence, kv head): its CTAs take every further group of pages, a warp
 // 256 / D pages at a time (D / 8 lanes a page, 8 dims each), and push the bounds into the first
@@ -243,12 +243,11 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
     for (int o = LR / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     top = all <= top ? top : all < INFINITY ? all : INFINITY;  // NaN too: nothing is then decided in fp32
 #pragma unroll
-    for (int j = 0; j < kKv4MaxGroup; ++j)
-      if (j < grp) {
+    for (int j = 0; j < kKv4MaxGroup; ++j) {  // all eight, in step: a branch at the group's end costs more
 #pragma unroll
-        for (int o = LR / 2; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-        best = fmaxf(best, s[j]);
-      }
+      for (int o = LR / 2; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+      if (j < grp) best = fmaxf(best, s[j]);
+    }
     if (pg < n - 1 && l == 0) {
       if (id < 0) {
         record_error(kDevBadPosition);
@@ -309,12 +308,13 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
     if (tid == 0) n_close = 0;
     __syncthreads();
     int* const close = reinterpret_cast<int*>(bound);  // their list takes the bounds' place, from below
+    int n_in = 0;
     for (int i0 = 0; i0 < n - 1; i0 += kKv4SelectThreads) {
       const int i = i0 + tid;
       const float v = i < n - 1 ? bound[i] : 0.f;
       const bool in = v > least + 2.f * off, out = v < least - 2.f * off;
       if (i < n - 1) exact[i] = in ? ~0ull : 0ull;
-      __syncthreads();  // these bounds have been read
+      n_in += __syncthreads_count(i < n - 1 && in);  // and these bounds have been read
       if (i < n - 1 && !in && !out) close[atomicAdd(&n_close, 1)] = i;
       __syncthreads();
     }
@@ -341,7 +341,23 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
       if (lane == 0) exact[i] = k;
     }
     __syncthreads();
-    t = kv4_nth([&](int i) { return exact[i]; }, n - 1, need, nth_s);
+    if (n_close <= kKv4SelectThreads) {  // each against the others: of those at hand need - n_in are taken
+      const int i = tid < n_close ? close[tid] : 0;
+      const unsigned long long k = exact[i];
+      int ahead = 0;
+      for (int c = 0; c < n_close; ++c) {
+        const unsigned long long o = exact[close[c]];
+        ahead += o > k || (o == k && close[c] < i);
+      }
+      __syncthreads();
+      if (tid < n_close) exact[i] = ahead < need - n_in ? ~0ull : 0ull;
+      __syncthreads();
+      t.at = ~0ull;
+      t.shift = 0;
+      t.left = need;
+    } else {
+      t = kv4_nth([&](int i) { return exact[i]; }, n - 1, need, nth_s);
+    }
   }
   // ---- in order: every thread a run of pages; above `at` all, at it the first `left`
   const int per = (n - 1 + kKv4SelectThreads - 1) / kKv4SelectThreads;

@@ -884,8 +884,9 @@ def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, ref
     need = _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, n_pages)
     # the workspace and the new rows are parts of one allocation
     extra = (need + 15) // 16 * 4 if workspace is None else 0
-    own, info, refs_out, lens_out, table_out = table.new_empty(extra + 4 + n_pages + batch + batch * max_pages).split(
-        (extra, 4, n_pages, batch, batch * max_pages))
+    own, info, refs_out, lens_out, table_out = table.new_empty(
+        extra + 4 + n_pages + batch + batch * max_pages).unsafe_split_with_sizes(
+            (extra, 4, n_pages, batch, batch * max_pages))
     ws, size = (own.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
     _kv4_call(dev, "b2_kv4_reorder", *args, pages, *rows, batch, max_pages, page, table_out.data_ptr(),
               lens_out.data_ptr(), refs_out.data_ptr(), info.data_ptr(), ws, size)
@@ -905,7 +906,7 @@ def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, 
     held = _kv4_need(refs, "refs", torch.int32, dev, (n_pages,))
     need = _kv4_ws_bytes(dev.index, "b2_kv4_compact_workspace_size", n_pages)
     extra = (need + 15) // 16 * 4 if workspace is None else 0
-    own, info, refs_out, table_out = table.new_empty(extra + 4 + n_pages + batch * max_pages).split(
+    own, info, refs_out, table_out = table.new_empty(extra + 4 + n_pages + batch * max_pages).unsafe_split_with_sizes(
         (extra, 4, n_pages, batch * max_pages))
     ws, size = (own.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
     _kv4_call(dev, "b2_kv4_compact", *args, pages, held, batch, max_pages, table_out.data_ptr(), refs_out.data_ptr(),
