@@ -360,9 +360,9 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.key_pages = pages;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
   // CTAs of a cluster: one per group of pages that its warps take at once, up to 8, and no more
-  // than the GPU holds in all (two per SM: 16 sequences x 8 kv heads of up to 1024 pages took
-  // 24.8 us so, and 32.6 in clusters of 8, which come in 3.5 waves)
-  const int group = b2::kKv4SelectThreads / 32 * (256 / head_dim);
+  // than the GPU holds in all, two per SM (16 sequences x 8 kv heads of 1024 pages: 17.6 us so,
+  // 23.3 at four per SM, 30.6 in clusters of 8)
+  const int group = b2::kKv4SelectThreads / 32 * 16;
   const long long pairs = static_cast<long long>(batch) * n_kv_heads;
   p.ctas = static_cast<int>(std::max(1LL, std::min({8LL, static_cast<long long>((pages + group - 1) / group), 2LL * di.sms / pairs})));
   const size_t smem = static_cast<size_t>(pages) * 12;

@@ -4,22 +4,27 @@
 //
 // lo and hi the page's key summary (per dim, over its tokens): but for the roundings of the
 // summary to bf16 and of the keys to 4 bits no token of the page scores higher with any of
-// the heads.  Per (sequence, kv head) the n_sel pages with the largest
-// bounds are listed, in ascending order of the page; the page of the query's own position
-// is always among them, and of two equal bounds the lower page goes first.
+// the heads.  Per (sequence, kv head) the n_sel pages with the largest bounds are listed, in
+// ascending order of the page; the page of the query's own position is always among them, and
+// of two equal bounds the lower page goes first.
 //
-// Which page is the n_sel-th may turn on the last bit of two bounds.  The bounds are summed in
-// fp32, with E, a bound on what that is off; where the last page taken and the first left out
-// are further apart than 2 E the choice is the exact one.  Where not (about one kv head in 300
-// of random keys; always with equal bounds), the pages within 2 E of the border are summed again in
-// fp64, with q turned in fp64 and the summaries bf16, every product exact, and chosen by that.
-// (In fp64 throughout 512 pages of 8 kv heads took 9.8 us, and 16 sequences of up to 1024 pages
-// 45 us; so 7.7 and 22.7.)
+// The bounds are products of a pages x 2 D matrix, the summaries as they lie in memory, with the
+// heads' min(q, 0) and max(q, 0), so the tensor cores take them: mma.sync m16n8k16 of bf16, q in
+// three parts that sum to its 24 bits, 16 pages x 8 heads a warp at a time (in fp32 on the other
+// pipes: 250 instructions for 4 pages and 22.6 us for 16 sequences x 8 kv heads of up to 1024
+// pages, against 14.8).
 //
-// A cluster per (sequence, kv head): its CTAs take every further group of pages, a warp
-// 256 / D pages at a time (D / 8 lanes a page, 8 dims each), and push the bounds into the first
-// CTA's shared memory, which finds the n_sel-th by 8-bit digits from the highest bit in which
-// they differ, until a digit settles it (two or three rounds), and writes the pages in order.
+// Which page is the n_sel-th may turn on the last bit of two bounds.  With E, a bound on what the
+// fp32 sums are off, the choice is the exact one where the last page taken and the first left out
+// are further apart than 2 E.  Where not (rarely with random keys; always with equal bounds), the
+// pages within 2 E of the border are summed again in fp64, with q turned in fp64 and the
+// summaries bf16, every product exact, and chosen by that.  (In fp64 throughout: 45 us.)
+//
+// A cluster per (sequence, kv head): its CTAs take every further group of pages and push the
+// bounds into the first CTA's shared memory, which finds the n_sel-th by 8-bit digits from the
+// highest bit in which they differ, until a digit settles it (two or three rounds), and writes
+// the pages in order.  That tail, 4 to 5 us of 7.6 for one sequence of 512 pages, is what bounds
+// a small call; the bytes of the summaries would take 2.5 of the 14.8 us.
 #pragma once
 
 #include "kv4_cell.cuh"
@@ -116,18 +121,26 @@ __device__ __forceinline__ Kv4Nth kv4_nth(const F& key, int n, int need, Kv4NthS
   return r;
 }
 
-// 8 bf16 pairs as they are stored (lo and hi of a lane's dims)
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// 64 dims of 16 pages' summaries as a warp holds them: of pages gl and gl + 8 (gl = lane / 4),
+// lo and hi, the 8 dims from 8 c and from 32 + 8 c on (c = lane % 4), bf16 as they are stored
 struct Kv4Near {
-  uint4 lo, hi;
+  uint4 v[2][2][2];
 };
 
 template <int D>
 __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const Kv4SelectParams p,
                                                                       const __grid_constant__ Kv4Rope rope) {
-  constexpr int LR = D / 8, RW = 32 / LR, W = kKv4SelectThreads / 32;
+  constexpr int G = D / 64, W = kKv4SelectThreads / 32;
   extern __shared__ __align__(16) unsigned long long exact[];  // [key_pages], then the fp32 bounds (the first CTA's)
   float* const bound = reinterpret_cast<float*>(exact + p.key_pages);
-  __shared__ __align__(16) float q_s[kKv4MaxGroup][D];
+  __shared__ uint2 qb[G][8][3][32];  // B operands: 64 dims; lo or hi, 16 dims; a bf16 part of q; lane
   __shared__ double turn_s[2][D / 2];
   __shared__ float size[W];
   __shared__ unsigned most;  // the largest sum_d qa |lo or hi| of a page, its bits (the first CTA's)
@@ -165,22 +178,24 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
     if (p.ctas > 1) cluster_wait_acquire();
     return;
   }
-  const int l = lane % LR, sub = lane / LR;
+  const int gl = lane >> 2, c = lane & 3;
   auto find = [&](int pg) { return pg < n - 1 ? kv4_page_id(p.table, p.max_pages, p.n_pages, b, pg) : -1; };
-  auto load = [&](int id, Kv4Near& x) {  // this lane's part of a page's summary
-    x.lo = x.hi = make_uint4(0, 0, 0, 0);
-    if (id >= 0) {
-      const __nv_bfloat16* sm = p.summary + (static_cast<size_t>(id) * p.hkv + kvh) * 2 * D + 8 * l;
-      x.lo = *reinterpret_cast<const uint4*>(sm);
-      x.hi = *reinterpret_cast<const uint4*>(sm + D);
+  auto load = [&](const int (&id)[2], int g, Kv4Near& x) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const __nv_bfloat16* sm = p.summary + (static_cast<size_t>(max(id[r], 0)) * p.hkv + kvh) * 2 * D + 64 * g + 8 * c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x.v[r][e >> 1][e & 1] = id[r] < 0 ? make_uint4(0, 0, 0, 0)
+                                          : *reinterpret_cast<const uint4*>(sm + (e >> 1) * D + 32 * (e & 1));
     }
   };
   // ---- the first pages' summaries set out; q turned to pos
-  const int step = p.ctas * W * RW;
-  int pg = (rank * W + warp) * RW + sub;
+  const int step = p.ctas * W * 16;
+  int pg = (rank * W + warp) * 16 + gl;  // and pg + 8
   Kv4Near x;
-  int id = find(pg), id_next = find(pg + step);
-  load(id, x);
+  int id[2] = {find(pg), find(pg + 8)}, id_next[2] = {find(pg + step), find(pg + step + 8)};
+  load(id, 0, x);
   if (rope.on) {
     for (int i = tid; i < D / 2; i += kKv4SelectThreads) {
       double u = static_cast<double>(pos) * kv4_turn(rope, i);
@@ -197,68 +212,87 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
     const double c = turn_s[0][i], s = turn_s[1][i];
     return second ? z * c + a * s : a * c - z * s;
   };
-  for (int e = tid; e < grp * (D / 2); e += kKv4SelectThreads) {
-    const int j = e / (D / 2), i = e % (D / 2);
-    q_s[j][i] = static_cast<float>(turned(j, i, false));
-    q_s[j][i + D / 2] = static_cast<float>(turned(j, i, true));
+  // the B operands: below zero for lo, above for hi, three bf16 that sum to q's 24 bits
+  float top = 0.f;
+  for (int e = tid; e < kKv4MaxGroup * (D / 4); e += kKv4SelectThreads) {
+    const int j = e % kKv4MaxGroup, d0 = e / kKv4MaxGroup * 4;
+    uint32_t w[2][3][2] = {};
+    if (j < grp) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + i;
+        float v = static_cast<float>(turned(j, d % (D / 2), d >= D / 2));
+        if (v != 0.f && fabsf(v) < 7.9e-31f) top = INFINITY;  // too small for the parts: all in fp64
+        const int side = v > 0.f;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const __nv_bfloat16 h = __float2bfloat16_rn(v);
+          v -= __bfloat162float(h);
+          w[0][k][i >> 1] |= side ? 0u : static_cast<uint32_t>(__bfloat16_as_ushort(h)) << (16 * (i & 1));
+          w[1][k][i >> 1] |= side ? static_cast<uint32_t>(__bfloat16_as_ushort(h)) << (16 * (i & 1)) : 0u;
+        }
+      }
+    }
+    const int at = d0 % 64, chunk = at / 8;  // chunk 4 i + c, its first or second half
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+        qb[d0 / 64][side * 4 + chunk / 4 * 2 + at / 4 % 2][k][j * 4 + chunk % 4] = make_uint2(w[side][k][0], w[side][k][1]);
   }
   __syncthreads();
-  // this lane's dims of every head, and the largest of the heads
-  float q[kKv4MaxGroup][8], qa[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    qa[i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kKv4MaxGroup; ++j) {
-      q[j][i] = j < grp ? q_s[j][8 * l + i] : 0.f;
-      qa[i] = fmaxf(qa[i], fabsf(q[j][i]));
-    }
-  }
   if (p.ctas > 1) cluster_wait_acquire();
-  // ---- the bounds in fp32: max(q lo, q hi) = q mid + |q| half
+  // ---- the bounds in fp32: 16 pages x 8 heads a warp at a time
   const uint32_t bound_s = smem_u32(bound);
-  float top = 0.f;
-  while (__any_sync(0xffffffffu, pg < n - 1)) {
-    Kv4Near y;
-    load(id_next, y);
-    const int id_after = find(pg + 2 * step);
-    float mid[8], half[8], s[kKv4MaxGroup], all = 0.f;  // all: of the products' sizes
-    const uint32_t lw[4] = {x.lo.x, x.lo.y, x.lo.z, x.lo.w}, hw[4] = {x.hi.x, x.hi.y, x.hi.z, x.hi.w};
+  while (pg - gl < n - 1) {
+    float s[4] = {}, low[4] = {}, all[4] = {};  // sums of q's first part, of the others, of the products' sizes
+    int id_after[2] = {find(pg + 2 * step), find(pg + 2 * step + 8)};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float lo = i % 2 ? bf16hi_to_f32(lw[i / 2]) : bf16lo_to_f32(lw[i / 2]);
-      const float hi = i % 2 ? bf16hi_to_f32(hw[i / 2]) : bf16lo_to_f32(hw[i / 2]);
-      mid[i] = 0.5f * hi + 0.5f * lo;
-      half[i] = 0.5f * hi - 0.5f * lo;
-      all = fmaf(qa[i], fabsf(mid[i]) + fabsf(half[i]), all);
-    }
+    for (int g = 0; g < G; ++g) {
+      Kv4Near y;
+      if (g + 1 < G) load(id, g + 1, y);
+      else load(id_next, 0, y);
 #pragma unroll
-    for (int j = 0; j < kKv4MaxGroup; ++j) {
-      s[j] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        const uint4 u = x.v[0][k >> 2][k >> 1 & 1], v = x.v[1][k >> 2][k >> 1 & 1];
+        const uint32_t a0 = k & 1 ? u.z : u.x, a1 = k & 1 ? v.z : v.x, a2 = k & 1 ? u.w : u.y, a3 = k & 1 ? v.w : v.y;
+        const uint2 b0 = qb[g][k][0][lane], b1 = qb[g][k][1][lane], b2 = qb[g][k][2][lane];
+        constexpr uint32_t kAbs = 0x7FFF7FFFu;
+        float first[4];  // summed outside: 16 products each stay near enough for E
+        mma_bf16_first(first, a0, a1, a2, a3, b0.x, b0.y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[j] = fmaf(q[j][i], mid[i], fmaf(fabsf(q[j][i]), half[i], s[j]));
-    }
-    float best = -INFINITY;
-#pragma unroll
-    for (int o = LR / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    top = all <= top ? top : all < INFINITY ? all : INFINITY;  // NaN too: nothing is then decided in fp32
-#pragma unroll
-    for (int j = 0; j < kKv4MaxGroup; ++j) {  // all eight, in step: a branch at the group's end costs more
-#pragma unroll
-      for (int o = LR / 2; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-      if (j < grp) best = fmaxf(best, s[j]);
-    }
-    if (pg < n - 1 && l == 0) {
-      if (id < 0) {
-        record_error(kDevBadPosition);
-        best = -INFINITY;
+        for (int e = 0; e < 4; ++e) s[e] += first[e];
+        mma_bf16_m16n8k16(low[0], low[1], low[2], low[3], a0, a1, a2, a3, b1.x, b1.y);
+        mma_bf16_m16n8k16(low[0], low[1], low[2], low[3], a0, a1, a2, a3, b2.x, b2.y);
+        mma_bf16_m16n8k16(all[0], all[1], all[2], all[3], a0 & kAbs, a1 & kAbs, a2 & kAbs, a3 & kAbs, b0.x & kAbs,
+                          b0.y & kAbs);
       }
-      if (p.ctas > 1) st_dsmem_f32(bound_s + pg * 4, 0, best);
-      else bound[pg] = best;
+      x = y;
     }
-    x = y;
-    id = id_next;
-    id_next = id_after;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float best = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (2 * c + e < grp) {
+          const float size = all[2 * r + e];
+          best = fmaxf(best, s[2 * r + e] + low[2 * r + e]);
+          top = size <= top ? top : size < INFINITY ? size : INFINITY;  // NaN too: nothing is then decided in fp32
+        }
+      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+      const int at = pg + 8 * r;
+      if (at < n - 1 && c == 0) {
+        if (id[r] < 0) {
+          record_error(kDevBadPosition);
+          best = -INFINITY;
+        }
+        if (p.ctas > 1) st_dsmem_f32(bound_s + at * 4, 0, best);
+        else bound[at] = best;
+      }
+      id[r] = id_next[r];
+      id_next[r] = id_after[r];
+    }
     pg += step;
   }
   top = warp_max(top);
@@ -282,9 +316,11 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
   }
   auto key = [&](int i) { return static_cast<unsigned long long>(kv4_key(bound[i])); };
   Kv4Nth t = kv4_nth(key, n - 1, need, nth_s);
-  // E: every lane's 16 products and the log2(D / 8) sums over lanes are rounded by 2^-24 of the
-  // sizes' sum at most, and so are q, mid and half; the sizes' own sum is fp32 too
-  const float off = __uint_as_float(most) * (28 * 5.9604644775390625e-8f);
+  // E: of 16 exact products, summed to single precision, each sum is off by 2^-23 of their sizes'
+  // sum at most; then D / 8 fp32 sums, half as much each.  The sizes' own sum is that of the first
+  // parts, within 1%; q's rounding, its other parts (4 D sums, 2^-9 as large) and the last sum are
+  // below 4 such roundings.
+  const float off = __uint_as_float(most) * ((16 + D / 16 + 4) * 1.02f * 1.1920929e-7f);
   float least = INFINITY, first_out = -INFINITY;  // of those taken, of those left out
   for (int i = tid; i < n - 1; i += kKv4SelectThreads) {
     if ((key(i) >> t.shift) >= t.at) least = fminf(least, bound[i]);
