@@ -92,7 +92,9 @@ class Q4Decoder:
                  weights: dict | None = None, gemm_min_batch: int = 9, pack_gemm: bool = True,
                  kv_cache: str = "bf16", kv_page: int = 64):
         """kv_cache: "bf16", dense caches of ctx_max positions; "kv4", 4-bit pages of kv_page
-        tokens (`cache`, a Kv4Cache with pages for ctx_max positions of every sequence)."""
+        tokens (`cache`, a Kv4Cache with pages for ctx_max positions of every sequence; a step
+        appends at `pos` and leaves cache.lens to its user, who sets them to pos + 1 before
+        the cache's rows are reordered)."""
         if kv_cache not in ("bf16", "kv4"):
             raise ValueError(f"kv_cache must be 'bf16' or 'kv4', got {kv_cache!r}")
         self.cfg = cfg

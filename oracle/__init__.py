@@ -20,4 +20,7 @@ gated attention decode steps) are restated in `deltanet_oracle.py` and
 from transformers' own modules (`tests/golden/make_deltanet_golden.py`,
 `make_gated_attn_golden.py`; `tests/test_deltanet_oracle.py`,
 `test_gated_attn_oracle.py`).
+
+The 4-bit paged KV cache has no counterpart in the reference: `kv4_oracle.py` states its
+definition in 64 bits (`tests/test_kv4_host.py` checks it against itself).
 """
