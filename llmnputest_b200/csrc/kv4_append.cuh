@@ -17,11 +17,12 @@
 // One CTA per (page of a sequence, kv head), so that the page's summary needs no second pass.
 // D / 8 lanes have a token, each two quads of dims (4 l and D / 2 + 4 l: the pairs that turn
 // together), so that what is done once per 64 values is done for 32 / (D / 8) tokens at a
-// time: 182 instructions a token and head of 64 dims, where a warp per token executed 282.  The
+// time: 182 instructions a token and head of 64 dims (before the codes were clamped and joined
+// by FMAs), where a warp per token executed 282.  The
 // codes are put together in shared memory as the cell's bytes.
 //
 // What bounds it: those instructions (2 x 64 values turned, compared and divided), at five CTAs
-// per SM.  8192 tokens of 8 heads of 64 in four prompts, appended and read back, take 29.5 us,
+// per SM.  8192 tokens of 8 heads of 64 in four prompts, appended and read back, take 28.6 us,
 // 9.2 by the bytes; one token for each of 64 sequences 8.8 us, two launches and their chains of
 // loads.  Six and eight CTAs per SM (fewer registers) measured no less.
 #pragma once
@@ -102,17 +103,20 @@ __device__ __forceinline__ uint32_t kv4_quantise(const X& x, const float (&f)[NV
   d = fmaxf(d, kKv4MinStep);
   float inv;
   asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(d));
-  // (x - m) / d, off by 2^-21 of what enters it at most, to the nearest whole number in the low
-  // bits of 3 * 2^22 + it; nearer than that to half a step between two, in fp64
-  const float near = 0.5f - fmaf(reach * inv, 4.8e-7f, 1e-5f), nm = -m * inv;
-  uint32_t code = 0;
-  float off = 0.f;
+  // (x - m) / d in fifteenths, off by 2^-21 of what enters it at most, clamped to 0..1 in the same
+  // instruction; 15 of it to the nearest whole number in the low bits of 3 * 2^22 + it.  Nearer
+  // than that to half a step between two, in fp64 (as where 1 / 15 d would be subnormal).
+  const float part = inv * (1.f / 15.f), nm = -m * part;
+  const float near = part > 1e-37f ? 0.5f - fmaf(reach * inv, 4.8e-7f, 1e-5f) : 0.f;
+  float off = 0.f, sum[NV / 4];  // sum: four codes, 2^23 + c0 + 16 c1 + ...
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const float z = fminf(fmaxf(fmaf(f[i], inv, nm), 0.f), 15.f), r = z + 12582912.f;
-    off = fmaxf(off, fabsf(z - (r - 12582912.f)));
-    code |= (__float_as_uint(r) & 15u) << (4 * i);
+    const float z = __saturatef(fmaf(f[i], part, nm)), t = fmaf(z, 15.f, 12582912.f) - 12582912.f;
+    off = fmaxf(off, fabsf(fmaf(z, 15.f, -t)));
+    sum[i / 4] = fmaf(t, static_cast<float>(1 << 4 * (i % 4)), i % 4 ? sum[i / 4] : 8388608.f);
   }
+  uint32_t code = NV == 8 ? prmt(__float_as_uint(sum[0]), __float_as_uint(sum[NV / 4 - 1]), 0x5410u)
+                          : __float_as_uint(sum[0]) & 0xFFFFu;
   const bool border = !(off < near);
   if (__any_sync(0xffffffffu, border)) {
     if (border) {

@@ -787,3 +787,22 @@ def test_decode_of_one_far_longer_sequence(ops, dim):
     for grp in (1, 8):
         got, ref = run_decode(ops, c, grp, rng, out_f32=True)
         close(host(got), ref, F32_TOL)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_values_of_any_size(ops, dim):
+    """Rows from fp32's subnormals to its largest, spreads far smaller than the values' own size,
+    and values on the very borders between codes."""
+    rng = np.random.default_rng(dim + 2)
+    n = 160
+    c = Case(rng, [n], 1, dim, 16, garbage=False)
+    size = 10.0 ** np.linspace(-44, 38, n)[:, None]
+    x = rng.uniform(-1, 1, (2, n, dim)) * size
+    x[:, 1::4] = size[1::4] * (1 + 1e-6 * rng.uniform(0, 1, (2, n // 4, dim)))
+    x[:, 2::4] = size[2::4] * rng.integers(0, 31, (2, n // 4, dim)) / 30
+    k, v = x.astype(np.float32)
+    c.cache.append(k, v, c.table, np.array([0]), np.array([0, n]), None)
+    ops.kv4_append(dev(k), dev(v), c.pool, c.dtable, dev(np.array([0], np.int32)),
+                   cu=dev(np.array([0, n], np.int32)), theta=None, summary=c.summary, **c.heads)
+    assert np.array_equal(host(c.pool), c.cache.pool())
+    assert np.array_equal(host(c.summary), c.cache.summary)
