@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
     }
     if (threadIdx.x == 0) {
       int2* span = p.spans + static_cast<size_t>(b) * p.hkv + kvh;
-      if (t_lo == 0) span->x = alone ? -1 : blockIdx.x;
+      if (t_lo == 0) span->x = alone ? -1 : static_cast<int>(blockIdx.x);
       if (t_hi == n_tiles) span->y = blockIdx.x;
     }
     if (!more) return;

@@ -334,7 +334,7 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   if (st != B2_OK) return st;
   st = kv4_decode_check({batch, n_kv_heads, head_dim, page, max_pages, n_pages}, n_q_heads, 0, max_len);
   if (st != B2_OK) return st;
-  int pages;
+  int pages = 0;
   st = kv4_select_check(page, n_sel, max_len, &pages);
   if (st != B2_OK) return st;
   if (!q || !summary || !table || !pos || !sel) return fail(B2_ERR_ARG, "null pointer argument");

@@ -806,3 +806,35 @@ def test_append_values_of_any_size(ops, dim):
                    cu=dev(np.array([0, n], np.int32)), theta=None, summary=c.summary, **c.heads)
     assert np.array_equal(host(c.pool), c.cache.pool())
     assert np.array_equal(host(c.summary), c.cache.summary)
+
+
+def test_two_graphs_of_one_pool(ops):
+    """Two captured calls that allocate their own workspaces, replayed in turn as positions and
+    queries change; tiles dealt over the grid, with pairs that several CTAs share."""
+    rng = np.random.default_rng(21)
+    lens = np.array([2500] * 20 + [1, 0, 777], np.int32)
+    c = Case(rng, lens, 8, 64, 64, garbage=False)
+    qs = [torch.zeros(len(lens), 8 * 64 * g, device="cuda") for g in (1, 5)]
+    graphs, outs = [], []
+
+    def call(i):
+        return ops.kv4_decode(qs[i], c.pool, c.dtable, c.pos, n_q_heads=qs[i].shape[1] // 64, out_f32=True, **c.heads)
+
+    for i in range(2):
+        call(i)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for turn in range(2):
+        at = np.maximum(lens - 1 - 300 * turn, np.minimum(lens - 1, 0)).astype(np.int32)
+        c.pos.copy_(dev(at))
+        x = [rng.standard_normal(tuple(q.shape)).astype(np.float32) for q in qs]
+        for q, y in zip(qs, x):
+            q.copy_(dev(y))
+        for i in (0, 1, 0):
+            graphs[i].replay()
+        for i in range(2):
+            want = c.cache.decode(x[i].reshape(len(lens), -1, 64), c.table, at, 10000.0).reshape(len(lens), -1)
+            close(host(outs[i]), want, F32_TOL, f"turn {turn} graph {i}")
