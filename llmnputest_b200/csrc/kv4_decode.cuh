@@ -14,6 +14,16 @@
 // S^T = K Q^T (16 tokens x 8 heads per instruction), O^T = V^T P^T; P moves from the
 // accumulator's layout to the B operand's with movmatrix.
 //
+// The fp16 weight w is off by up to 2^-11 of the fp32 one, u, and the tensor cores' fp32 sums are
+// truncated, not rounded.  Both would add up over a long sequence, as codes are never negative
+// (32 sequences of 32768 equal scores: 8e-3 of the output's norm), so sums are kept around zero:
+//   out = sum w (c - 7.5) + sum p (f + 7.5 e),  sum w (c - 7.5) = sum w c - 7.5 sum w,
+// the last sum in fp32; and every other tile enters negated, as (-w) (15 - c), whose like sum is
+// sum (-w) (15 - c) - 7.5 sum (-w).  What stays is one rounding of a weight against half the
+// range of the values (that case: 2.0e-4; random queries over 512 to 32768 tokens 2.7e-4 to
+// 3.0e-4, half of it q's rounding, and 4.1e-4 to 6.4e-4 with the plain sums).  64 sequences of
+// 4096 take 39.5 us so and took 37.5; with a product by -7.5 after each one instead, 43.4.
+//
 // Weights are taken against a running reference R per head (log2 units) instead of the
 // running maximum: w = 2^(s - R) e goes into the product as fp16, R is raised, and the sums
 // rescaled, only when some w passes 2^10.  R covers s + log2 e, so that w keeps fp16's 11
@@ -157,8 +167,8 @@ template <int D>
 struct Kv4State {
   static constexpr int G = D / kKv4Group;
   float o[G][4][4];   // O^T accumulators of group g, rows 8 (lane / 4) + i and + 4: even i the sum of
-                      // w a (dim i), odd i that of w (a + 16 b) (dims i - 1 and i)
-  float m[G][2];      // sum p f
+                      // w a (dim i), odd i that of w (a + 16 b) (dims i - 1 and i), negated tiles as said
+  float m[G][2];      // sum p (f + 7.5 e) - 7.5 w, w negated with its tile
   float l[2], r[2];
 };
 
@@ -180,6 +190,13 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// m - 7.5 w, w an fp16, in one rounding
+__device__ __forceinline__ float kv4_less_middle(uint32_t w, float m) {
+  float d;
+  asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(static_cast<uint16_t>(w)), "h"(static_cast<uint16_t>(0xC780u)), "f"(m));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t f16x2_max_nan(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -187,9 +204,9 @@ __device__ __forceinline__ uint32_t f16x2_max_nan(uint32_t a, uint32_t b) {
 }
 
 // NT tiles of 16 tokens; the G cells of tile n start at tile0 + n * stride.  MASK: only
-// left[n] of its tokens count.
+// left[n] of its tokens count.  index: the first tile's place in its stage; odd ones are negated.
 template <int D, int NT, bool MASK>
-__device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, const int* left,
+__device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int index, const int* left,
                                           const uint32_t (&qb)[D / 64][4][2], const float (&qs)[D / 64][2],
                                           const float (&unit)[2], Kv4State<D>& st) {
   constexpr int G = D / kKv4Group;
@@ -294,13 +311,22 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, cons
   for (int n = 0; n < NT; ++n) {
     st.l[0] += pr[n][0] + pr[n][2];
     st.l[1] += pr[n][1] + pr[n][3];
+    const uint32_t negate = (index + n) & 1 ? 0xFFFFFFFFu : 0u;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float f0 = bf16hi_to_f32(vm[n][g].x), f1 = bf16hi_to_f32(vm[n][g].y);
+      const float f0 = fmaf(7.5f, bf16lo_to_f32(vm[n][g].x), bf16hi_to_f32(vm[n][g].x));
+      const float f1 = fmaf(7.5f, bf16lo_to_f32(vm[n][g].y), bf16hi_to_f32(vm[n][g].y));
       st.m[g][0] = fmaf(pr[n][0], f0, fmaf(pr[n][2], f1, st.m[g][0]));
       st.m[g][1] = fmaf(pr[n][1], f0, fmaf(pr[n][3], f1, st.m[g][1]));
-      const uint32_t b0 = movmatrix_trans(w[n][g][0]), b1 = movmatrix_trans(w[n][g][1]);
-      const uint4 v = *reinterpret_cast<const uint4*>(tile0 + n * stride + g * kKv4CellBytes + kKv4VCodes + gl * 64 + c * 16);
+      const uint32_t w0 = w[n][g][0] ^ (negate & 0x80008000u), w1 = w[n][g][1] ^ (negate & 0x80008000u);
+      st.m[g][0] = kv4_less_middle(w0 & 0xFFFFu, kv4_less_middle(w1 & 0xFFFFu, st.m[g][0]));
+      st.m[g][1] = kv4_less_middle(w0 >> 16, kv4_less_middle(w1 >> 16, st.m[g][1]));
+      const uint32_t b0 = movmatrix_trans(w0), b1 = movmatrix_trans(w1);
+      uint4 v = *reinterpret_cast<const uint4*>(tile0 + n * stride + g * kKv4CellBytes + kKv4VCodes + gl * 64 + c * 16);
+      v.x ^= negate;
+      v.y ^= negate;
+      v.z ^= negate;
+      v.w ^= negate;
       float(&o)[4][4] = st.o[g];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {  // bytes 0 and 2, then 1 and 3: the same dims of two tokens
@@ -627,11 +653,11 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
       if (whole >> slot & 1) {
 #pragma unroll
         for (int n = 0; n < ST; n += NT)
-          kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, nullptr, qb, qs, unit, st);
+          kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, nullptr, qb, qs, unit, st);
       } else {
 #pragma unroll 1
         for (int n = 0; n < 1 << run.lg; n += NT)
-          kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, &left_s[warp][slot][n], qb, qs, unit, st);
+          kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, &left_s[warp][slot][n], qb, qs, unit, st);
       }
       __syncwarp();  // every lane has read the slot
       if (issued < run.n_stages) issue();
