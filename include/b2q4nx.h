@@ -442,8 +442,10 @@ int b2_kv4_gather(void* k, void* v, int64_t ld_k, int64_t ld_v, int rows, const 
  * entry that is negative, behind pos[b] or not above the entry before it counts for
  * nothing.  Without sel, n_sel is 0.  max_len >= max(pos) + 1 sizes the split.
  * q enters the products as fp16 (scaled by a power of two per head), the weights as fp16
- * against fp32 sums.  Scores beyond 10^8 in size want V's steps d below 2^15.  workspace:
- * 16-byte aligned; calls that may run at the same time need one each. */
+ * against fp32 sums: each is off by 2^-11 of itself at most, every head's 64 dims by about
+ * 3e-4 of their size and by no more for long sequences.  Values up to 2^60 in size; scores
+ * beyond 10^8 in size want V's steps d below 2^15.  workspace: 16-byte aligned; calls that
+ * may run at the same time need one each. */
 int b2_kv4_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page, int n_sel,
                                  int max_len, size_t* bytes);
 int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32_t* table, const int32_t* pos,

@@ -26,9 +26,13 @@
 //
 // Weights are taken against a running reference R per head (log2 units) instead of the
 // running maximum: w = 2^(s - R) e goes into the product as fp16, R is raised, and the sums
-// rescaled, only when some w passes 2^10.  R covers s + log2 e, so that w keeps fp16's 11
-// bits whatever the size of the values; the sums L = sum 2^(s - R) and sum 2^(s - R) f stay
-// in fp32.
+// rescaled, only when some w passes 2^10.  R covers s + log2 e of the largest e of a token's
+// groups of 64 dims.  A group whose own largest weight then lies below 2^-10 is weighed in a unit
+// of its own, a power of two by head and group that its sums carry to the end, so that its w keep
+// fp16's bits too: rare in earnest, so tiles are first taken as if all units were 1 (256 sequences
+// of 2048 of 256 dims 75.9 us so, 73.5 without units, 79.0 with them in every tile).  The sums
+// L = sum 2^(s - R) and sum 2^(s - R) f stay in fp32; with the least e, 2^-40, the weights 2^(s - R)
+// reach 2^50, and f may be 2^60 in size.
 #pragma once
 
 #include "kv4_cell.cuh"
@@ -172,6 +176,10 @@ struct Kv4State {
   float l[2], r[2];
 };
 
+// A group whose largest weight is not below this is weighed as it is: 2^-15 of that weight is
+// then what fp16's subnormals lose.
+constexpr float kKv4NearOne = 0x1p-10f;
+
 // Orders this thread's accesses to shared memory before later bulk copies into it.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -180,6 +188,11 @@ __device__ __forceinline__ float kv4_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 1 over the power of two at or below x (2^-60 <= x <= 2^60)
+__device__ __forceinline__ float kv4_power_inv(float x) {
+  return __uint_as_float(0x7F000000u - (__float_as_uint(x) & 0x7F800000u));
 }
 
 // A B with nothing to add to.
@@ -203,12 +216,16 @@ __device__ __forceinline__ uint32_t f16x2_max_nan(uint32_t a, uint32_t b) {
   return d;
 }
 
-// NT tiles of 16 tokens; the G cells of tile n start at tile0 + n * stride.  MASK: only
-// left[n] of its tokens count.  index: the first tile's place in its stage; odd ones are negated.
-template <int D, int NT, bool MASK>
-__device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int index, const int* left,
+// NT tiles of 16 tokens; the G cells of tile n start at tile0 + n * stride.  index: the first
+// tile's place in its stage; odd ones are negated.
+// ANY: only left[n] of a tile's tokens count, and the groups' units (times; scaled: some are not
+// 1) are set as they have to be; returns whether they are all 1.  Else the tiles are full and the
+// units 1; where one has to be set the sums are left as they were, against the R raised, and the
+// tiles are to be taken again (false; again: these are such).
+template <int D, int NT, bool ANY>
+__device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int index, const int* left,
                                           const uint32_t (&qb)[D / 64][4][2], const float (&qs)[D / 64][2],
-                                          const float (&unit)[2], Kv4State<D>& st) {
+                                          const float (&unit)[2], float (*times)[kKv4MaxGroup], bool scaled, bool again, Kv4State<D>& st) {
   constexpr int G = D / kKv4Group;
   constexpr uint32_t kLo = 0x000F000Fu;
   const int lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
@@ -239,7 +256,7 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int 
       y[n][2] = fmaf(d1, a[2], fmaf(m1, qs[g][0], y[n][2]));
       y[n][3] = fmaf(d1, a[3], fmaf(m1, qs[g][1], y[n][3]));
     }
-    if (MASK) {  // what lies behind the last token may hold anything
+    if (ANY) {  // what lies behind the last token may hold anything
       constexpr uint32_t kNothing = 0x2B80u;  // e = 2^-40, f = 0
       if (gl >= left[n]) {
         y[n][0] = y[n][1] = -INFINITY;
@@ -255,29 +272,34 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int 
   }
   float pr[NT][4];
   uint32_t w[NT][G][2];  // the weights of heads 2c, 2c + 1, for token gl and token gl + 8
-  // weights against the present R; whether one of them has come to 2^10, or is not a number.
-  // Against a new R the scores are rounded as they were for it: past 2^27 an unrounded product
-  // may lie further above R than fp16 reaches.
-  auto weigh = [&](bool anew) -> bool {
-    uint32_t top = 0;
+  // weights against the present R (weigh) and the groups' units (pack); whether one of them has
+  // come to 2^10, or is not a number.  Against a new R the scores are rounded as they were for it:
+  // past 2^27 an unrounded product may lie further above R than fp16 reaches.
+  auto weigh = [&](bool anew) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         pr[n][i] = kv4_ex2(anew ? __fmul_rn(y[n][i], unit[i & 1]) - st.r[i & 1] : fmaf(y[n][i], unit[i & 1], -st.r[i & 1]));
+  };
+  auto pack = [&]() -> bool {
+    uint32_t top = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float e0 = bf16lo_to_f32(vm[n][g].x), e1 = bf16lo_to_f32(vm[n][g].y);
-        w[n][g][0] = pack_f16x2(pr[n][0] * e0, pr[n][1] * e0);
-        w[n][g][1] = pack_f16x2(pr[n][2] * e1, pr[n][3] * e1);
+        const float u0 = ANY && G > 1 && scaled ? times[g][2 * c] : 1.f, u1 = ANY && G > 1 && scaled ? times[g][2 * c + 1] : 1.f;
+        w[n][g][0] = pack_f16x2(pr[n][0] * u0 * e0, pr[n][1] * u1 * e0);
+        w[n][g][1] = pack_f16x2(pr[n][2] * u0 * e1, pr[n][3] * u1 * e1);
         top = f16x2_max_nan(top, f16x2_max_nan(w[n][g][0], w[n][g][1]));
       }
-    }
     return (top + 0x1C001C00u) & 0x80008000u;  // 0x6400 is 2^10
   };
-  if (__any_sync(0xffffffffu, weigh(false))) {
+  weigh(false);
+  if (__any_sync(0xffffffffu, pack()) || again) {
     // raise R to the largest s + log2 e seen, and rescale what has been summed against the old one
-    float r[2] = {-INFINITY, -INFINITY};
+    float r[2] = {-INFINITY, -INFINITY}, fall[2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -292,20 +314,67 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int 
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) r[i] = fmaxf(r[i], __shfl_xor_sync(0xffffffffu, r[i], o));
       r[i] = fmaxf(r[i], st.r[i]);
-      const float f = kv4_ex2(st.r[i] - r[i]);
+      fall[i] = kv4_ex2(st.r[i] - r[i]);
       st.r[i] = r[i];
-      st.l[i] *= f;
+      st.l[i] *= fall[i];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        st.m[g][i] *= f;
+        st.m[g][i] *= fall[i];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          st.o[g][k][i] *= f;
-          st.o[g][k][i + 2] *= f;
+          st.o[g][k][i] *= fall[i];
+          st.o[g][k][i + 2] *= fall[i];
         }
       }
     }
     weigh(true);
+    if (G > 1) {  // does every group have a weight near 1, for every head?
+      auto most = [&](int g, int i) {
+        float x = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          x = fmaxf(x, fmaxf(pr[n][i] * bf16lo_to_f32(vm[n][g].x), pr[n][i + 2] * bf16lo_to_f32(vm[n][g].y)));
+        return x;
+      };
+      bool near = !scaled;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float x = most(g, i);
+          const unsigned large = __ballot_sync(0xffffffffu, x >= kKv4NearOne);
+          near = near && (large >> c & 0x11111111u) != 0 && x < 2.f;
+        }
+      if (!__all_sync(0xffffffffu, near)) {
+        if (!ANY) return false;
+        bool one = true;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = most(g, i);
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const float old = times[g][2 * c + i];
+            x = fmaxf(x, fall[i] * kv4_power_inv(old));  // or the largest that it had
+            float now = x >= kKv4NearOne && x < 2.f ? 1.f : kv4_power_inv(fminf(fmaxf(x, 0x1p-60f), 0x1p60f));
+            if (st.r[i] == kKv4NoScore) now = old;  // no score yet
+            one = one && now == 1.f;
+            const float f = now * kv4_power_inv(old);
+            st.m[g][i] *= f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              st.o[g][k][i] *= f;
+              st.o[g][k][i + 2] *= f;
+            }
+            __syncwarp();
+            times[g][2 * c + i] = now;  // the same from all lanes of the head
+          }
+        __syncwarp();
+        scaled = !__all_sync(0xffffffffu, one);
+      }
+    }
+    pack();
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -316,8 +385,9 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int 
     for (int g = 0; g < G; ++g) {
       const float f0 = fmaf(7.5f, bf16lo_to_f32(vm[n][g].x), bf16hi_to_f32(vm[n][g].x));
       const float f1 = fmaf(7.5f, bf16lo_to_f32(vm[n][g].y), bf16hi_to_f32(vm[n][g].y));
-      st.m[g][0] = fmaf(pr[n][0], f0, fmaf(pr[n][2], f1, st.m[g][0]));
-      st.m[g][1] = fmaf(pr[n][1], f0, fmaf(pr[n][3], f1, st.m[g][1]));
+      const float u0 = ANY && G > 1 && scaled ? times[g][2 * c] : 1.f, u1 = ANY && G > 1 && scaled ? times[g][2 * c + 1] : 1.f;
+      st.m[g][0] = fmaf(pr[n][0] * u0, f0, fmaf(pr[n][2] * u0, f1, st.m[g][0]));
+      st.m[g][1] = fmaf(pr[n][1] * u1, f0, fmaf(pr[n][3] * u1, f1, st.m[g][1]));
       const uint32_t w0 = w[n][g][0] ^ (negate & 0x80008000u), w1 = w[n][g][1] ^ (negate & 0x80008000u);
       st.m[g][0] = kv4_less_middle(w0 & 0xFFFFu, kv4_less_middle(w1 & 0xFFFFu, st.m[g][0]));
       st.m[g][1] = kv4_less_middle(w0 >> 16, kv4_less_middle(w1 >> 16, st.m[g][1]));
@@ -337,7 +407,9 @@ __device__ __forceinline__ void kv4_tiles(const uint8_t* tile0, int stride, int 
       }
     }
   }
+  return ANY ? !scaled : true;
 }
+
 
 __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, int head, int D, int d, float v) {
   const size_t i = static_cast<size_t>(b) * p.ldo + static_cast<size_t>(head) * D + d;
@@ -411,6 +483,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
   __shared__ __align__(8) uint64_t full[W][NS];
   __shared__ int left_s[W][NS][ST];
   __shared__ float mr[W][kKv4MaxGroup], ml[W][kKv4MaxGroup];
+  __shared__ float times_s[W][G][kKv4MaxGroup];  // D > 64: what a group's weights in o and m are multiplied by
   __shared__ int area[kArea];  // dealt: weights of the sequences below; cluster: what the CTAs push
   __shared__ int abort_flag, scan[W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
@@ -607,7 +680,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
       if (lane == 0) mbar_arrive_expect_tx(bar, __popc(some >> o & tiles) * Ring::kTileBytes);
       __syncwarp();
       if (mine < 1u << run.lg) {
-        if (!all) left_s[warp][in_slot][mine] = left_now & ~kBehind;
+        left_s[warp][in_slot][mine] = left_now & ~kBehind;
         if (copy_bytes)
           bulk_g2s(ring_s + in_slot * Ring::kStageBytes + mine * Ring::kTileBytes, at_now, copy_bytes, bar, once);
       }
@@ -640,6 +713,9 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
     }
     st.l[0] = st.l[1] = 0.f;
     st.r[0] = st.r[1] = kKv4NoScore;
+    if (G > 1 && lane < G * kKv4MaxGroup) times_s[warp][lane / kKv4MaxGroup][lane % kKv4MaxGroup] = 1.f;
+    __syncwarp();
+    bool scaled = false;  // some group's unit is not 1
 
     int done = 0;
     for (; done < run.n_stages; ++done) {
@@ -650,15 +726,21 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
         if (!__all_sync(0xffffffffu, here)) break;
       }
       const uint8_t* stage = ring + slot * Ring::kStageBytes;
-      if (whole >> slot & 1) {
+      int n = 0;
+      bool again = false;
+      if (!scaled && whole >> slot & 1) {
 #pragma unroll
-        for (int n = 0; n < ST; n += NT)
-          kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, nullptr, qb, qs, unit, st);
-      } else {
-#pragma unroll 1
-        for (int n = 0; n < 1 << run.lg; n += NT)
-          kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, &left_s[warp][slot][n], qb, qs, unit, st);
+        for (; n < ST; n += NT)
+          if (!kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, nullptr, qb, qs, unit, nullptr,
+                                       scaled, false, st)) {
+            again = true;
+            break;
+          }
       }
+#pragma unroll 1
+      for (; n < 1 << run.lg; n += NT, again = false)
+        scaled = !kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, &left_s[warp][slot][n], qb, qs,
+                                         unit, times_s[warp], scaled, again, st);
       __syncwarp();  // every lane has read the slot
       if (issued < run.n_stages) issue();
       if (++slot == NS) {
@@ -713,7 +795,8 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float sum = i & 1 ? st.o[g][i][e] - st.o[g][i - 1][e] : st.o[g][i][e];
-          mo[warp][2 * c + (e & 1)][64 * g + 8 * gl + 2 * (e & 2) + i] = fmaf(sum, scale, st.m[g][e & 1]);
+          const float back = G > 1 ? kv4_power_inv(times_s[warp][g][2 * c + (e & 1)]) : 1.f;
+          mo[warp][2 * c + (e & 1)][64 * g + 8 * gl + 2 * (e & 2) + i] = fmaf(sum, scale, st.m[g][e & 1]) * back;
         }
       }
     if (p.splits > 1) cluster_wait_acquire();  // the cluster's CTAs have all begun

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import kv4_oracle as kv4
-from tests.test_gpu_kv4 import dev, host, no_device_error, ops  # noqa: F401  (fixtures)
+from tests.test_gpu_kv4 import F32_TOL, Case, dev, host, no_device_error, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,60 @@ def test_long_sequences_of_equal_scores(ops, steps):
                          out_f32=True)
     off = np.abs(host(got) - want).max()
     assert off <= tol, f"{off:.3g} > {tol:.3g}"
+
+
+def by_group(x, dim):
+    return np.linalg.norm(np.asarray(x, np.float64).reshape(-1, dim // 64, 64), axis=-1)
+
+
+def decode_by_group(ops, c, grp, seed, tol):
+    """Every head's 64 dims on their own: off by tol of their 2-norm at most."""
+    b, hq = len(c.lens), grp * c.hkv
+    q = np.random.default_rng(seed).standard_normal((b, hq * c.dim)).astype(np.float32)
+    ref = c.cache.decode(q.reshape(b, hq, c.dim), c.table, c.lens - 1, 10000.0)
+    got = host(ops.kv4_decode(dev(q), c.pool, c.dtable, c.pos, n_q_heads=hq, out_f32=True, **c.heads))
+    assert np.isfinite(got).all()
+    off, size = by_group(got.reshape(ref.shape) - ref, c.dim), by_group(ref, c.dim)
+    worst = (off / np.maximum(size, 1e-300))[size > 0].max()
+    assert worst <= tol, f"{worst:.3g} > {tol:.3g}"
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("power", [0, -9, -12, -20, -30])
+def test_groups_of_unlike_size(ops, dim, power):
+    """V's groups of 64 dims 2^power of one another: each of them as near as one alone is (3
+    roundings of 2^-11: q's, the weights', and both in the sum that they are divided by)."""
+    rng = np.random.default_rng(dim - power)
+    c = Case(rng, [1, 17, 64, 100, 33], 2, dim, 32)
+    size = 2.0 ** (power * (np.arange(dim // 64) % 2))
+    size[-1] = 2.0 ** power
+    c.cache.meta[..., 1, :, :] *= size[:, None, None]
+    c.pool = dev(c.cache.pool())
+    decode_by_group(ops, c, 4, 1, F32_TOL)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_groups_whose_size_changes(ops, dim):
+    """Groups that are small at first and large later, or the other way round, or in one page
+    alone, in sequences that one warp reads whole and that many share."""
+    rng = np.random.default_rng(dim)
+    c = Case(rng, [900, 64, 16, 500], 2, dim, 16, garbage=False)
+    for b, n in enumerate(c.lens):
+        pages = -(-int(n) // 16)
+        for i, at in enumerate(c.table[b, :pages]):
+            for g in range(dim // 64):
+                power = [(-25, 0), (0, -25), (0, 0), (-25, 12)][(b + g) % 4][int(2 * i >= pages)]
+                c.cache.meta[at, :, :, g, 1] *= 2.0 ** power
+    c.pool = dev(c.cache.pool())
+    decode_by_group(ops, c, 3, 2, F32_TOL)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_constant_values(ops, dim):
+    """Tokens whose values are all alike have the least step, 2^-40, however large they are."""
+    rng = np.random.default_rng(dim)
+    c = Case(rng, [40, 17, 300], 2, dim, 16, garbage=False)
+    c.cache.meta[..., 0, 1, :, 0] = 2.0 ** -40
+    c.cache.meta[..., 0, 1, :, 1] = kv4.bf16(1e17 * (1 + rng.random(c.cache.meta.shape[:3] + (16,))))
+    c.pool = dev(c.cache.pool())
+    decode_by_group(ops, c, 2, 3, F32_TOL)
