@@ -7,15 +7,19 @@
     for l in range(n_layers): cache.append(l, k, v, pos, cu=cu)       # prompts, ragged
     cache.advance(prompt_lens)
     ...
-    cache.reserve(1)                                 # a decode step: one more token a row
+    cache.reserve(1)                                 # a decode step: one more token a row in use
+    pos = cache.positions()                          # -1 for the others
     for l in ...: cache.append(l, k, v, pos); out = cache.decode(l, q, pos, n_q_heads=40)
     cache.advance(1)
-    cache.reorder(parent)                            # beams, new requests, rows that ended
+    cache.reorder(parent)                            # beams, rows that ended (-1)
+    cache.reorder(same, reserve)                     # a request into a row that ended: its pages
 
 A value takes 4.5 bits (codes of 4 bits, a bf16 step and least value per token, kv head and
 64 dims) where the dense cache of `ops.gqa_decode` takes 16.  Rows share full pages; the table
 and its counts live on the device and nothing here waits for it: `info` of the last reorder or
-compact can be read when a host wants to know what is free.  The buffers stay where they are,
+compact can be read when a host wants to know what is free.  A row that a reorder emptied is not
+in use until one reserves pages for it: it takes no page and no token of reserve(1) and
+advance(1), and attends to nothing.  The buffers stay where they are,
 so a captured step sees what later calls put into them.  No reference counterpart (the reference
 keeps one sequence's K and V in bf16, designs/granite_gemv/granite_attention.h:80-213)."""
 
@@ -47,6 +51,10 @@ class Kv4Cache:
         self.lens = torch.zeros(batch, **i32)
         self.refs = torch.zeros(n_pages, **i32)
         self.info = torch.zeros(4, **i32)
+        # 1 for a row in use; one more entry, 0, for those that go on with no row
+        self._use = torch.ones(batch + 1, **i32)
+        self._use[batch] = 0
+        self.used = self._use[:batch]
         self._same = torch.arange(batch, **i32)
         self._layers = list(self.pool.unbind(0))
         self._near = list(self.summary.unbind(0)) if summaries else [None] * n_layers
@@ -57,21 +65,35 @@ class Kv4Cache:
 
     def reorder(self, parent: torch.Tensor, reserve: torch.Tensor | None = None) -> torch.Tensor:
         """Row b goes on with the tokens of row parent[b] (-1: with none), and has pages for
-        reserve[b] more (ops.kv4_reorder).  Returns info: free pages left, pages copied, pages
-        missing, 0."""
+        reserve[b] more (ops.kv4_reorder).  The row is in use if row parent[b] was, or if
+        reserve[b] is above 0.  Returns info: free pages left, pages copied, pages missing, 0."""
+        self._rows(parent, reserve)
+        self.used.copy_(self._use[parent.clamp(-1, self.batch)])  # -1 and batch: the entry that is 0
+        if reserve is not None:
+            self.used.logical_or_(reserve > 0)
+        return self.info
+
+    def _rows(self, parent: torch.Tensor, reserve: torch.Tensor | None) -> None:
         table, lens, refs, info = ops.kv4_reorder(self.pool, self.table, self.lens, self.refs, parent,
                                                   head_dim=self.head_dim, reserve=reserve, summary=self.summary)
         self.table.copy_(table)
         self.lens.copy_(lens)
         self.refs.copy_(refs)
         self.info.copy_(info)
-        return self.info
 
     def reserve(self, tokens: int | torch.Tensor) -> torch.Tensor:
-        """Pages for that many tokens behind those that every row has (int32 [batch], or one number)."""
-        if not isinstance(tokens, torch.Tensor):
-            tokens = torch.full_like(self.lens, int(tokens))
-        return self.reorder(self._same, tokens)
+        """Pages for that many tokens behind those that a row has: int32 [batch] (a row with more
+        than 0 is in use from then on), or one number for every row in use."""
+        if isinstance(tokens, torch.Tensor):
+            self._rows(self._same, tokens)
+            self.used.logical_or_(tokens > 0)
+        else:
+            self._rows(self._same, self.used * int(tokens))
+        return self.info
+
+    def positions(self) -> torch.Tensor:
+        """Where every row's next token goes: int32 [batch], -1 for a row that is not in use."""
+        return torch.where(self.used > 0, self.lens, -1)
 
     def compact(self) -> torch.Tensor:
         """Live pages to the lowest numbers (ops.kv4_compact).  Returns info: live pages, pages moved, 0, 0."""
@@ -82,8 +104,12 @@ class Kv4Cache:
         return self.info
 
     def advance(self, tokens: int | torch.Tensor) -> None:
-        """The rows have that many more tokens (what has been appended to every layer)."""
-        self.lens.add_(tokens)
+        """The rows have that many more tokens, what has been appended to every layer (int32
+        [batch], or one number for every row in use)."""
+        if isinstance(tokens, torch.Tensor):
+            self.lens.add_(tokens)
+        else:
+            self.lens.add_(self.used, alpha=int(tokens))
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, *,
                cu: torch.Tensor | None = None, theta: float | None = 10000.0) -> None:
