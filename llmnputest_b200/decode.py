@@ -93,8 +93,7 @@ class Q4Decoder:
                  kv_cache: str = "bf16", kv_page: int = 64):
         """kv_cache: "bf16", dense caches of ctx_max positions; "kv4", 4-bit pages of kv_page
         tokens (`cache`, a Kv4Cache with pages for ctx_max positions of every sequence; a step
-        appends at `pos` and leaves cache.lens to its user, who sets them to pos + 1 before
-        the cache's rows are reordered)."""
+        appends at `pos` and leaves cache.lens alone; `reorder` forks and ends sequences)."""
         if kv_cache not in ("bf16", "kv4"):
             raise ValueError(f"kv_cache must be 'bf16' or 'kv4', got {kv_cache!r}")
         self.cfg = cfg
@@ -195,6 +194,20 @@ class Q4Decoder:
         ops.gemv_rmsnorm(self.w["lm_head"], self.nt_v, self.kt_h, self.resid, self.w["final_norm"], c.rms_eps,
                          out=self.logits, prefetch=prefetch, q8=True)
         return self.logits
+
+    def reorder(self, parent: torch.Tensor) -> None:
+        """Sequence b goes on as sequence parent[b] (int32 [batch]; -1: it ends) stands after a
+        step at `pos` (kv_cache="kv4"): its cached tokens, with pages for ctx_max positions, and
+        its `pos` (-1 where it ended: the next request's first token goes to 0).  `pos` and the
+        cache's buffers stay where they are, so a captured step goes on with the new rows."""
+        if self.cache is None:
+            raise ValueError("reorder needs kv_cache='kv4'")
+        c = self.cache
+        torch.add(self.pos, 1, out=c.lens)
+        # a row is given what it needs up to ctx_max again: a fork its own pages behind the copied one
+        kept = torch.cat([c.lens, c.lens.new_zeros(1)])[parent.clamp(-1, self.batch)]
+        c.reorder(parent, self.ctx_max - kept)
+        torch.sub(c.lens, 1, out=self.pos)
 
     def _attend(self, li: int, prefetch: bool) -> None:
         """attn = layer li's attention on the rows of qkv, whose k and v join its cache at `pos`."""

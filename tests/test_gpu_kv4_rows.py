@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import kv4_oracle as kv4
-from tests.test_gpu_kv4 import F32_TOL, close, dev, host, no_device_error, ops  # noqa: F401  (fixtures)
+from tests.test_gpu_kv4 import BF16_TOL, F32_TOL, close, dev, host, no_device_error, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +145,55 @@ def test_captured_steps_of_a_served_cache(ops):
             s.reorder([-1, 1])
     assert (out[0] == 0).all()
     del g
+
+
+@pytest.mark.parametrize("batch,captured", [(3, False), (3, True), (12, True)])
+def test_decoder_forks_and_ends(ops, batch, captured):
+    """A decoder's sequences fork in the middle of a page and at its end, end and begin anew, and
+    step on to ctx_max: the cache and the attention of every step against the oracle's, on the
+    step's own projections."""
+    from llmnputest_b200 import decode
+    cfg = decode.DecoderConfig(n_layers=1, hidden=512, n_heads=8, n_kv_heads=2, intermediate=512, vocab=1024)
+    ctx, page = 50, 16
+    dec = decode.Q4Decoder(cfg, batch, ctx, seed=5, kv_cache="kv4", kv_page=page)
+    rng = np.random.default_rng(batch)
+    graph = dec.capture() if captured else None
+    rows = [[] for _ in range(batch)]
+    pos = np.zeros(batch, np.int32)
+    pos[-1] = -1  # a padded sequence at first
+    forks = {20: [0, 0, -1], 31: [1, 0, 0], 40: [0, -1, 2]}  # (page ends at 16, 32, 48)
+    for t in range(ctx):
+        dec.pos.copy_(dev(pos))
+        dec.x_in.copy_(dev(rng.standard_normal((batch, cfg.hidden))))
+        graph.replay() if captured else dec.step()
+        qkv, got = host(dec.qkv), host(dec.attn)
+        for b in range(batch):
+            if pos[b] < 0:
+                assert (got[b] == 0).all()
+                continue
+            rows[b].append(qkv[b, 512:])
+            n = len(rows[b])
+            assert n == pos[b] + 1
+            kv, pages = np.stack(rows[b]), -(-n // page)
+            ref, table = kv4.Cache(pages, 2, 64, page), np.arange(pages)[None]
+            ref.append(kv[:, :128], kv[:, 128:], table, [0], [0, n], cfg.rope_theta)
+            want = ref.decode(qkv[b, :512].reshape(1, 8, 64), table, [n - 1], cfg.rope_theta)
+            close(got[b:b + 1], want.reshape(1, -1), BF16_TOL, f"step {t} sequence {b}")
+        if t in forks:
+            parent = np.array((forks[t] + list(range(3, batch)))[:batch], np.int32)
+            dec.reorder(dev(parent))
+            assert host(dec.cache.info)[2] == 0
+            rows = [list(rows[p]) if p >= 0 else [] for p in parent]
+            assert host(dec.pos).tolist() == [len(r) - 1 for r in rows] == (host(dec.cache.lens) - 1).tolist()
+        pos = np.minimum(np.array([len(r) for r in rows]), ctx - 1).astype(np.int32)
+        pos[[len(r) == ctx for r in rows]] = -1
+        if t < 45:
+            pos[-1] = -1 if batch > 3 or t < 20 else pos[-1]
+    del graph
+
+
+def test_decoder_reorder_is_refused_without_pages(ops):
+    from llmnputest_b200 import decode
+    cfg = decode.DecoderConfig(n_layers=1, hidden=512, n_heads=8, n_kv_heads=2, intermediate=512, vocab=1024)
+    with pytest.raises(ValueError, match="kv4"):
+        decode.Q4Decoder(cfg, 1, 16).reorder(dev(np.zeros(1, np.int32)))
