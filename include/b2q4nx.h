@@ -405,8 +405,8 @@ int b2_q4_gemm_swiglu_in(const uint8_t* tiles, int n_tile_rows, int k_tiles, con
  *   pos      int32 [batch], as in b2_gqa_decode; -1 marks a sequence without tokens (a
  *            padded batch row)
  *   head_dim 64, 128 or 256; n_q_heads / n_kv_heads <= 8.
- * A position outside the table, or an entry outside the pool where a page is needed,
- * records device error 5; nothing is read or written for it.  Device error 7: the pool
+ * A position outside the table or not below max_len (decode without sel, select), or an
+ * entry outside the pool where a page is needed, records device error 5; nothing is read or written for it.  Device error 7: the pool
  * had no free page left (b2_kv4_reorder). */
 #define B2_KV4_NO_ROPE 1  /* keys or queries are not rotated */
 #define B2_KV4_OUT_F32 2  /* b2_kv4_decode: fp32 output */

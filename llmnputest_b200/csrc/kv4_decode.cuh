@@ -56,7 +56,7 @@ struct Kv4DecodeParams {
   long long ldo;
   float scale_log2;
   int batch, hq, hkv, page, max_pages, n_pages, n_sel;
-  int max_tiles;  // tiles of the longest sequence planned for
+  int max_len;    // tokens of the longest sequence planned for (without sel)
   int splits;     // CTAs of a (sequence, kv head), a cluster; 0: the tiles are dealt over the grid
   int2* spans;    // [batch][hkv] the CTAs that share a pair, or x = -1 (dealt over the grid)
   int out_f32;
@@ -459,7 +459,7 @@ constexpr int kKv4MaxDealt = 1024;  // sequences of a launch whose tiles are dea
 // Tiles of sequence b: 0 where it has no token, or (reported by the caller) a bad position.
 __device__ __forceinline__ int kv4_seq_tiles(const Kv4DecodeParams& p, int pos, bool& bad) {
   bad = pos < -1 || pos >= static_cast<long long>(p.max_pages) * p.page ||
-        (!p.sel && pos >= p.max_tiles * static_cast<long long>(kKv4Tile));
+        (!p.sel && pos >= p.max_len);
   if (bad || pos < 0) return 0;
   return p.sel ? p.n_sel * (p.page / kKv4Tile) : pos / kKv4Tile + 1;
 }

@@ -266,7 +266,7 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
   p.n_pages = n_pages;
   p.n_sel = n_sel;
   p.splits = pl.splits;
-  p.max_tiles = pl.tiles;
+  p.max_len = max_len;
   p.out_f32 = (flags & B2_KV4_OUT_F32) ? 1 : 0;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
   cudaError_t e = kv4_by_dim(head_dim, [&](auto d) {
@@ -357,6 +357,7 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.max_pages = max_pages;
   p.n_pages = n_pages;
   p.n_sel = n_sel;
+  p.max_len = max_len;
   p.key_pages = pages;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
   // CTAs of a cluster: one per group of pages that its warps take at once, up to 8, and no more

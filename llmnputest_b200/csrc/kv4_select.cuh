@@ -39,7 +39,8 @@ struct Kv4SelectParams {
   const int* pos;
   int* sel;  // [batch][hkv][n_sel]
   int batch, hq, hkv, page, max_pages, n_pages, n_sel;
-  int key_pages;  // pages planned for (max_len)
+  int max_len;    // tokens planned for
+  int key_pages;  // in pages
   int ctas;       // of a cluster
 };
 
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads, 2) kv4_select_kernel(const 
   pdl_launch_dependents();
   int* sel = p.sel + (static_cast<size_t>(b) * p.hkv + kvh) * p.n_sel;
   const int pos = p.pos[b];
-  if (pos < 0 || pos >= static_cast<long long>(p.max_pages) * p.page || pos / p.page >= p.key_pages) {
+  if (pos < 0 || pos >= static_cast<long long>(p.max_pages) * p.page || pos >= p.max_len) {
     if (rank == 0) {
       if (pos != -1 && tid == 0) record_error(kDevBadPosition);
       for (int i = tid; i < p.n_sel; i += kKv4SelectThreads) sel[i] = -1;

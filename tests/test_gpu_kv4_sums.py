@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import kv4_oracle as kv4
-from tests.test_gpu_kv4 import F32_TOL, Case, dev, host, no_device_error, ops  # noqa: F401  (fixtures)
+from tests.test_gpu_kv4 import F32_TOL, Case, close, dev, host, no_device_error, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,29 @@ def test_long_sequences_of_equal_scores(ops, steps):
                          out_f32=True)
     off = np.abs(host(got) - want).max()
     assert off <= tol, f"{off:.3g} > {tol:.3g}"
+
+
+@pytest.mark.parametrize("batch", [1, 70])
+def test_positions_past_the_planned_length(ops, batch):
+    """max_len bounds pos + 1 to the token, not to its tile or page: a position past it is reported
+    and left alone, one below it is not touched by that; in a cluster and with tiles dealt out."""
+    rng = np.random.default_rng(batch)
+    c = Case(rng, [100] * batch, 8, 64, 64)
+    q = dev(rng.standard_normal((batch, 8 * 64)))
+    call = dict(n_q_heads=8, theta=None, max_len=99)
+    for last, bad in ((98, False), (99, True)):
+        pos = np.full(batch, 98, np.int32)
+        pos[0] = last
+        out = torch.full((batch, 512), 3.0, device="cuda")
+        ops.kv4_decode(q, c.pool, c.dtable, dev(pos), out=out, out_f32=True, **call, **c.heads)
+        assert ops.device_error() == (5 if bad else 0)
+        want = c.cache.decode(host(q).reshape(batch, 8, 64), c.table, pos).reshape(batch, -1)
+        rest = slice(1 if bad else 0, None)
+        close(host(out)[rest], want[rest], F32_TOL)
+        assert (out[0] == 3.0).all() or not bad
+        sel = ops.kv4_select(q, c.summary, c.dtable, dev(pos), page=64, n_sel=2, **call, **c.heads)
+        assert ops.device_error() == (5 if bad else 0)
+        assert (sel[0] == -1).all() or not bad
 
 
 def by_group(x, dim):
