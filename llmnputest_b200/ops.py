@@ -668,9 +668,11 @@ def _kv4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> tuple[int, 
 
 
 def _kv4_call(device: torch.device, name: str, *args) -> None:
-    """A call on `device`'s current stream, whichever device is current."""
+    """A call on `device`'s current stream, whichever device is current.  The raw stream is asked
+    for as torch does for its own generated code: 0.07 us, where building a Stream takes 1.3 of a
+    call's 13."""
     index = device.index
-    if torch._C._cuda_getDevice() != index:
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
             return _kv4_call(device, name, *args)
     status = getattr(_native._LIB or _native.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
