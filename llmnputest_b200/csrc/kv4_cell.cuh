@@ -98,14 +98,10 @@ __device__ __forceinline__ void kv4_rows(const int* cu, int rows, int b, int& lo
 }
 
 // The job-th (sequence, page) that a ragged batch touches, for a warp: returns the
-// sequence, or -1 behind the last; first = the page's index in its sequence.
+// sequence, or -1 behind the last; pg = the page's index in its sequence.
 __device__ __forceinline__ int kv4_find_job(const int* cu, const int* pos, int rows, int batch, int page, int job,
                                             int& pg) {
   const int lane = threadIdx.x & 31;
-  if (!cu) {
-    pg = job < batch ? max(pos[job], 0) / page : 0;
-    return job < batch ? job : -1;
-  }
   for (int b0 = 0; b0 < batch; b0 += 32) {
     const int b = b0 + lane;
     int n = 0, first = 0;

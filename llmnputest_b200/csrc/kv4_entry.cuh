@@ -424,10 +424,10 @@ int b2_kv4_copy_pages(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64
   return B2_OK;
 }
 
-// need, copy, totals, then the free pages found
+// need, copy, the number of free pages found, then those
 static size_t kv4_reorder_ws(int batch, int max_pages, int n_pages) {
   const size_t ids = std::min(static_cast<size_t>(batch) * max_pages, static_cast<size_t>(n_pages));
-  return (2 * static_cast<size_t>(batch) + 2 + ids) * sizeof(int);
+  return (2 * static_cast<size_t>(batch) + 1 + ids) * sizeof(int);
 }
 
 int b2_kv4_reorder_workspace_size(int batch, int max_pages, int n_pages, size_t* bytes) {
@@ -466,8 +466,8 @@ int b2_kv4_reorder(uint8_t* pool, int64_t page_bytes, uint8_t* summary, int64_t 
   p.info = info;
   p.need = static_cast<int*>(workspace);
   p.copy = p.need + batch;
-  p.totals = p.copy + batch;
-  p.free_ids = p.totals + 2;
+  p.n_found = p.copy + batch;
+  p.free_ids = p.n_found + 1;
   p.batch = batch;
   p.max_pages = max_pages;
   p.page = page;

@@ -52,7 +52,7 @@ struct Kv4ReorderParams {
   int* need;  // [batch] pages each row lacks, then their sums below each row
   int* copy;  // [batch] 0, or 1 + which of the row's missing pages is a copy of its parent's last one
   int* free_ids;  // [total needed] at most batch * max_pages
-  int* totals;    // [2]: pages needed, pages found
+  int* n_found;   // how many of them there are
   int batch, max_pages, page;
 };
 
@@ -166,8 +166,7 @@ __global__ void __launch_bounds__(kKv4PlanThreads) __cluster_dims__(kKv4PlanCtas
       below += sum;
     }
     if (tid == 0) {
-      p.totals[0] = total;
-      p.totals[1] = min(all, total);
+      *p.n_found = min(all, total);
       p.info[0] = all - min(all, total);
       if (all < total) {
         record_error(kDevNoPage);
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(kKv4CopyThreads) kv4_reorder_fill_kernel(const
   const int b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  const int found = p.totals[1], rank0 = p.need[b];
+  const int found = *p.n_found, rank0 = p.need[b];
   const int par = p.parent[b];
   const int copy_rank = rank0 + p.copy[b] - 1;
   const bool copies = p.copy[b] != 0;
