@@ -8,23 +8,25 @@
 //   gather  code * d + m of the rows asked for.
 //
 // The codes are whole numbers that turn on the last bit of x at a border between two of
-// them, and are to be the same whatever the order of evaluation.  So keys are turned in fp64
-// (as fast as integer work here: a complex multiplication a token by the angle of four
-// positions, from one sincospi a page), and every choice is made in fp32 with a bound on its
+// them, and are to be the same whatever the order of evaluation.  So keys are turned in fp64: a
+// lane's first token by its own sine and cosine, every further one by a complex multiplication
+// with the turn of the positions between the two (16 at head_dim 64, 8 at 128, 4 at 256), whose
+// sine and cosine are evaluated once a page.  Every choice is made in fp32 with a bound on its
 // error; the few that lie within the bound of a border (1 in 10^4 or less) are made again in
 // fp64.
 //
 // One CTA per (page of a sequence, kv head), so that the page's summary needs no second pass.
 // D / 8 lanes have a token, each two quads of dims (4 l and D / 2 + 4 l: the pairs that turn
 // together), so that what is done once per 64 values is done for 32 / (D / 8) tokens at a
-// time: 182 instructions a token and head of 64 dims (before the codes were clamped and joined
-// by FMAs), where a warp per token executed 282.  The
+// time: 168 instructions a token and head of 64 dims, where a warp per token executed 282.  The
 // codes are put together in shared memory as the cell's bytes.
 //
-// What bounds it: those instructions (2 x 64 values turned, compared and divided), at five CTAs
-// per SM.  8192 tokens of 8 heads of 64 in four prompts, appended and read back, take 28.6 us,
-// 9.2 by the bytes; one token for each of 64 sequences 8.8 us, two launches and their chains of
-// loads.  Six and eight CTAs per SM (fewer registers) measured no less.
+// What bounds it: those instructions and their latency (2 x 64 values turned, compared and
+// divided; under half of the issue slots are used), in two rounds of CTAs, four per SM.  8192
+// tokens of 8 heads of 64 in four prompts, appended and read back, take 27.7 us, 9.2 by the
+// bytes; one token for each of 64 sequences 8.4 us, two launches and their chains of loads.
+// Five CTAs per SM spill registers (24 to 60 bytes): 28.6 us, and 36.6 against 32.8 for 4096
+// tokens of 8 heads of 128; six and eight measured no less than five.
 #pragma once
 
 #include "kv4_cell.cuh"
@@ -165,7 +167,7 @@ __device__ __forceinline__ void kv4_load4(const char* src, bool f32, bool wide, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kKv4AppendThreads, 5) kv4_append_kernel(const Kv4RowsParams p,
+__global__ void __launch_bounds__(kKv4AppendThreads, 4) kv4_append_kernel(const Kv4RowsParams p,
                                                                           const __grid_constant__ Kv4Rope rope) {
   constexpr int G = D / kKv4Group, W = kKv4AppendThreads / 32;
   constexpr int LR = D / 8, RW = 32 / LR, STEP = W * RW;  // lanes of a token, tokens of a warp, of the CTA
