@@ -220,12 +220,11 @@ __device__ __forceinline__ uint32_t f16x2_max_nan(uint32_t a, uint32_t b) {
 // tile's place in its stage; odd ones are negated.
 // ANY: only left[n] of a tile's tokens count, and the groups' units (times; scaled: some are not
 // 1) are set as they have to be; returns whether they are all 1.  Else the tiles are full and the
-// units 1; where one has to be set the sums are left as they were, against the R raised, and the
-// tiles are to be taken again (false; again: these are such).
+// units 1; where one has to be set nothing is done (false).
 template <int D, int NT, bool ANY>
 __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int index, const int* left,
                                           const uint32_t (&qb)[D / 64][4][2], const float (&qs)[D / 64][2],
-                                          const float (&unit)[2], float (*times)[kKv4MaxGroup], bool scaled, bool again, Kv4State<D>& st) {
+                                          const float (&unit)[2], float (*times)[kKv4MaxGroup], bool scaled, Kv4State<D>& st) {
   constexpr int G = D / kKv4Group;
   constexpr uint32_t kLo = 0x000F000Fu;
   const int lane = threadIdx.x & 31, gl = lane >> 2, c = lane & 3;
@@ -297,9 +296,10 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
     return (top + 0x1C001C00u) & 0x80008000u;  // 0x6400 is 2^10
   };
   weigh(false);
-  if (__any_sync(0xffffffffu, pack()) || again) {
+  if (__any_sync(0xffffffffu, pack())) {
     // raise R to the largest s + log2 e seen, and rescale what has been summed against the old one
     float r[2] = {-INFINITY, -INFINITY}, fall[2];
+    const float before[2] = {st.r[0], st.r[1]};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -316,16 +316,6 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
       r[i] = fmaxf(r[i], st.r[i]);
       fall[i] = kv4_ex2(st.r[i] - r[i]);
       st.r[i] = r[i];
-      st.l[i] *= fall[i];
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        st.m[g][i] *= fall[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          st.o[g][k][i] *= fall[i];
-          st.o[g][k][i + 2] *= fall[i];
-        }
-      }
     }
     weigh(true);
     if (G > 1) {  // does every group have a weight near 1, for every head?
@@ -346,7 +336,11 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
           near = near && (large >> c & 0x11111111u) != 0 && x < 2.f;
         }
       if (!__all_sync(0xffffffffu, near)) {
-        if (!ANY) return false;
+        if (!ANY) {
+          st.r[0] = before[0];
+          st.r[1] = before[1];
+          return false;
+        }
         bool one = true;
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -372,6 +366,19 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
           }
         __syncwarp();
         scaled = !__all_sync(0xffffffffu, one);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      st.l[i] *= fall[i];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        st.m[g][i] *= fall[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          st.o[g][k][i] *= fall[i];
+          st.o[g][k][i + 2] *= fall[i];
+        }
       }
     }
     pack();
@@ -727,20 +734,17 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
       }
       const uint8_t* stage = ring + slot * Ring::kStageBytes;
       int n = 0;
-      bool again = false;
       if (!scaled && whole >> slot & 1) {
 #pragma unroll
         for (; n < ST; n += NT)
           if (!kv4_tiles<D, NT, false>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, nullptr, qb, qs, unit, nullptr,
-                                       scaled, false, st)) {
-            again = true;
+                                       scaled, st))
             break;
-          }
       }
 #pragma unroll 1
-      for (; n < 1 << run.lg; n += NT, again = false)
+      for (; n < 1 << run.lg; n += NT)
         scaled = !kv4_tiles<D, NT, true>(stage + n * Ring::kTileBytes, Ring::kTileBytes, n, &left_s[warp][slot][n], qb, qs,
-                                         unit, times_s[warp], scaled, again, st);
+                                         unit, times_s[warp], scaled, st);
       __syncwarp();  // every lane has read the slot
       if (issued < run.n_stages) issue();
       if (++slot == NS) {

@@ -197,3 +197,27 @@ def test_decoder_reorder_is_refused_without_pages(ops):
     cfg = decode.DecoderConfig(n_layers=1, hidden=512, n_heads=8, n_kv_heads=2, intermediate=512, vocab=1024)
     with pytest.raises(ValueError, match="kv4"):
         decode.Q4Decoder(cfg, 1, 16).reorder(dev(np.zeros(1, np.int32)))
+
+
+def test_captured_reorders(ops):
+    """A reorder and a reserve captured once and replayed with other parents."""
+    s = Served(batch=3)
+    s.prompts([20, 5, 33])
+    parent, more = dev(np.array([0, 1, 2], np.int32)), dev(np.zeros(3, np.int32))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s.c.reorder(parent, more)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        s.c.reorder(parent, more)
+    for new, reserve in (([0, 0, -1], [0, 3, 0]), ([1, -1, 0], [1, 0, 1]), ([0, 2, 2], [0, 0, 0])):
+        parent.copy_(dev(np.array(new, np.int32)))
+        more.copy_(dev(np.array(reserve, np.int32)))
+        g.replay()
+        s.rows = [list(s.rows[p]) if p >= 0 else [] for p in new]
+        alive = {b for b, r in enumerate(s.rows) if r}
+        assert s.c.used.tolist() == [int(b in alive) for b in range(3)]
+        s.step(alive)
+    del g

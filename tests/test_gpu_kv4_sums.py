@@ -124,3 +124,39 @@ def test_constant_values(ops, dim):
     c.cache.meta[..., 0, 1, :, 1] = kv4.bf16(1e17 * (1 + rng.random(c.cache.meta.shape[:3] + (16,))))
     c.pool = dev(c.cache.pool())
     decode_by_group(ops, c, 2, 3, F32_TOL)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("each", ["group", "page"])
+def test_groups_of_unlike_size_in_shared_pairs(ops, dim, each):
+    """The same with every pair's tiles dealt over several CTAs, in full stages, whose parts are
+    joined; one group small throughout, or every page's groups of a size of their own."""
+    rng = np.random.default_rng(dim + 1)
+    c = Case(rng, rng.integers(1, 700, 150), 2, dim, 64, garbage=False)
+    if each == "group":
+        power = -18.0 * (np.arange(dim // 64) % 2)
+    else:
+        power = rng.choice([0, -18, -30, 10], (len(c.cache.meta), 1, 1, dim // 64))
+    c.cache.meta[..., 1, :, :] *= 2.0 ** power[..., None, None]
+    c.pool = dev(c.cache.pool())
+    decode_by_group(ops, c, 2, 4, F32_TOL)
+
+
+@pytest.mark.parametrize("power", [0, -20])
+def test_nan_with_groups(ops, power):
+    """A NaN key spoils its own sequence and kv head, a NaN value its own 64 dims; nothing else."""
+    rng = np.random.default_rng(power + 30)
+    c = Case(rng, [70, 70, 70], 2, 128, 16)
+    c.cache.meta[..., 1, 1, :, :] *= 2.0 ** power
+    c.cache.meta[c.table[0, 1], 0, 0, 1, 0, 3, 1] = np.nan
+    c.cache.meta[c.table[1, 3], 1, 0, 1, 1, 9, 1] = np.nan
+    c.pool = dev(c.cache.pool())
+    q = rng.standard_normal((3, 4 * 128)).astype(np.float32)
+    ref = c.cache.decode(q.reshape(3, 4, 128), c.table, c.lens - 1).reshape(3, 2, 2, 2, 64)
+    got = host(ops.kv4_decode(dev(q), c.pool, c.dtable, c.pos, n_q_heads=4, theta=None, out_f32=True,
+                              **c.heads)).reshape(ref.shape)
+    assert np.isnan(got[0, 0]).all() and np.isnan(got[1, 1, :, 1]).all()
+    ok = np.isfinite(ref)
+    assert np.isfinite(got[ok]).all() and ok.sum() == ref.size - 2 * 128 - 2 * 64
+    off, size = by_group(np.where(ok, got - ref, 0.0), 64), by_group(np.where(ok, ref, 0.0), 64)
+    assert (off <= F32_TOL * size).all()
