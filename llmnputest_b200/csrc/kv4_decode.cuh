@@ -22,7 +22,7 @@
 // sum (-w) (15 - c) - 7.5 sum (-w).  What stays is one rounding of a weight against half the
 // range of the values (that case: 2.0e-4; random queries over 512 to 32768 tokens 2.7e-4 to
 // 3.0e-4, half of it q's rounding, and 4.1e-4 to 6.4e-4 with the plain sums).  64 sequences of
-// 4096 take 39.5 us so and took 37.5; with a product by -7.5 after each one instead, 43.4.
+// 4096 take 39.4 us so and took 37.5; with a product by -7.5 after each one instead, 43.4.
 //
 // Weights are taken against a running reference R per head (log2 units) instead of the
 // running maximum: w = 2^(s - R) e goes into the product as fp16, R is raised, and the sums
@@ -30,7 +30,7 @@
 // groups of 64 dims.  A group whose own largest weight then lies below 2^-10 is weighed in a unit
 // of its own, a power of two by head and group that its sums carry to the end, so that its w keep
 // fp16's bits too: rare in earnest, so tiles are first taken as if all units were 1 (256 sequences
-// of 2048 of 256 dims 75.9 us so, 73.5 without units, 79.0 with them in every tile).  The sums
+// of 2048 of 256 dims 75.5 us so, 73.5 without units, 79.0 with them in every tile).  The sums
 // L = sum 2^(s - R) and sum 2^(s - R) f stay in fp32; with the least e, 2^-40, the weights 2^(s - R)
 // reach 2^50, and f may be 2^60 in size.
 #pragma once
@@ -432,18 +432,22 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
 //   whole ones and the beginning of another, and a second kernel joins the pairs that were
 //   cut.  (One grid row of CTAs per pair left SMs without work at lengths of 1 to 4096, and
 //   every wave of CTAs after the first costs its start and end again.)
-// Inside a CTA the stages of a pair go to the warps in turn; a stage is 4608 bytes (two tiles,
-// 9216, at D = 256: 70.4 us against 74.5 at 256 sequences of 2048), or fewer tiles where warps
-// would be left without one.  Every warp fills a ring of its own with bulk copies, one per
+// Inside a CTA the stages of a pair go to the warps in turn; a stage is 4608 bytes (at D = 256
+// 9216, two tiles, of which one enters negated), or fewer tiles where warps would be left
+// without one.  Every warp fills a ring of its own with bulk copies, one per
 // run of tiles that lie in a row, and looks the pages up 32 tiles at a time.
 //
-// What bounds it: instruction issue and the latency of a tile's chain (products, exponentials,
-// products) with 8 to 16 warps per SM.  64 sequences x 8 kv heads of 4096 tokens (152 MB of
-// cache, 23.2 us at the measured HBM rate) take 37.4 us, 4.1 TB/s; 256 x 2 of 2048 tokens of 256
-// dims (305 MB, 46.5 us) 70.1 us, 4.3 TB/s.  With a tile's arithmetic left out the rest takes
-// 28.5 and 53.8, with the copies left out 34.8 and 66.8.  Measured and dropped: stages
-// of half the size (43 us at D = 64), three stages, 5 to 8 CTAs per SM (registers spill), one
-// tile or four at a time, a tile's scores beside the values of the one before.
+// What bounds it: the latency of a tile's chain (products, exponentials, products) with 8 to 16
+// warps per SM; 55% of the issue slots, 48% of the ALU pipe and 44% of DRAM are used.  64
+// sequences x 8 kv heads of 4096 tokens (152 MB of cache, 23.2 us at the measured HBM rate) take
+// 39.4 us, 3.9 TB/s; 64 x 8 of 2048 of 128 dims (152 MB) 42.5; 256 x 2 of 2048 of 256 dims (305
+// MB, 46.5 us) 75.5 us, 4.0 TB/s.  With a tile's arithmetic left out the rest takes 28.4, 30.1
+// and 57.5; with the copies left out the first takes 37.9.  Measured and dropped, at these three:
+// stages of half the size 45.2, 45.4 and 75.5; three stages (fewer CTAs per SM) 48.7, 56.2 and
+// 113.8; 5 to 8 CTAs per SM (registers spill); a tile's scores beside the values of the one
+// before.  At D = 64 two tiles are taken at a time (one: 40.4), at 128 one (two: 43.6); at 256
+// one takes 254 registers.  At 128 four CTAs per SM spill 112 bytes, three with 168 registers
+// none: 48.6, though 20.2 against 22.0 for 16 sequences of 1 to 4096.
 constexpr int kKv4RunOverhead = 32;
 template <int D>
 struct Kv4Ring {
@@ -452,8 +456,8 @@ struct Kv4Ring {
   static constexpr int kTiles = D == 256 ? 2 : 4 / G;  // tiles of a stage at most
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kTiles * kTileBytes;
-  // what a run costs beside its tiles, its start and end, in tiles of a CTA (16 at D = 64
-  // measured 1.2 us slower at 16 sequences of 1 to 4096 tokens)
+  // what a run costs beside its tiles, its start and end, in tiles of a CTA (16 sequences of 1 to
+  // 4096 tokens, D = 64: 32 tiles 15.8 us, 16 16.0; D = 128: 16 22.0, 8 23.6 to 23.9, 32 22.1)
   static constexpr int kOverhead = kKv4RunOverhead / G;
 };
 template <int D, int W>
@@ -876,7 +880,7 @@ __global__ void __launch_bounds__(W * 32, D == 256 ? 2 : 4) kv4_decode_kernel(co
 
 // Joins the pairs that several CTAs share, and clears the rows of sequences without tokens:
 // grid (kv head, sequence, share of the heads).  A thread joins four outputs of one head (one
-// each, at D = 64: 20.7 us against 15.0 for one sequence of 32768); threads beyond the outputs
+// each, at D = 64: 20.7 us where four took 15.0 for one sequence of 32768); threads beyond the outputs
 // take every further part of them (many parts a pair).
 // The parts' loads set out together: the kernel is two trips to L2 long.
 constexpr int kKv4JoinMost = 512;

@@ -91,8 +91,8 @@ struct Kv4DecodePlan {
 };
 
 // A cluster per (sequence, kv head) while the clusters fit the GPU at once and no warp has more
-// than 16 tiles (one sequence, 8 kv heads of 64: 10.9 us against 13.5 dealt at 16384 tokens,
-// but two of 32768 21.8 against 18.0, and one with 128 dims 26.4 against 21.3); else the tiles
+// than 16 tiles (one sequence, 8 kv heads of 64: 11.3 us against 13.6 dealt at 16384 tokens,
+// but two of 32768 22.4 against 18.5, and one of 32768 with 128 dims 27.8 against 20.9); else the tiles
 // are dealt over as many CTAs as the GPU holds, each with two per warp at least.
 Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int tokens, int sms) {
   Kv4DecodePlan pl = {};
@@ -105,8 +105,8 @@ Kv4DecodePlan kv4_decode_plan(int batch, int hq, int hkv, int head_dim, int toke
     return pl;
   }
   // a whole number of CTAs a pair, or of pairs a CTA, where that leaves few slots empty: equal
-  // lengths are then not cut (64 sequences x 8 kv heads of 4096 tokens: 37.4 us with 512 CTAs,
-  // 40.8 with all 592)
+  // lengths are then not cut (64 sequences x 8 kv heads of 4096 tokens: 39.4 us with 512 CTAs,
+  // 46 with all 592)
   long long n = slots;
   if (pairs <= slots) {
     if (slots / pairs * pairs * 10 >= slots * 8) n = slots / pairs * pairs;
@@ -303,8 +303,8 @@ int b2_kv4_decode(const float* q, int64_t ld_q, const uint8_t* pool, const int32
       cudaError_t r = cudaLaunchKernelEx(&l.cfg, kernel, part, rope);
       if (r != cudaSuccess) return r;
       // few pairs with many parts each: a CTA per head, up to 16 threads to an output's parts (8
-      // sequences x 8 kv heads of 8192: 18.5 us against 21.4 with a CTA per kv head, but 16 of
-      // 4096, with 4.6 parts a pair, 19.9 against 17.1)
+      // sequences x 8 kv heads of 8192: 19.0 us against 21.7 with a CTA per kv head, but 16 of
+      // 4096, with 4.6 parts a pair, 20.5 against 17.7)
       const int grp = n_q_heads / n_kv_heads;
       const bool few = pl.ctas > 8 * part.batch * n_kv_heads;
       Kv4Launch j(dim3(n_kv_heads, part.batch, few ? grp : 1), few ? std::min(4 * D, b2::kKv4JoinMost) : grp * D / 4, stream);
@@ -361,8 +361,8 @@ int b2_kv4_select(const float* q, int64_t ld_q, const uint16_t* summary, const i
   p.key_pages = pages;
   const b2::Kv4Rope& rope = kv4_rope(theta, head_dim, flags);
   // CTAs of a cluster: one per group of pages that its warps take at once, up to 8, and no more
-  // than the GPU holds in all, two per SM (16 sequences x 8 kv heads of 1024 pages: 17.6 us so,
-  // 23.3 at four per SM, 30.6 in clusters of 8)
+  // than the GPU holds in all, two per SM (16 sequences x 8 kv heads of up to 1024 pages: 13.9 us
+  // so, 19.8 at four per SM, 26.7 in clusters of 8)
   const int group = b2::kKv4SelectThreads / 32 * 16;
   const long long pairs = static_cast<long long>(batch) * n_kv_heads;
   p.ctas = static_cast<int>(std::max(1LL, std::min({8LL, static_cast<long long>((pages + group - 1) / group), 2LL * di.sms / pairs})));

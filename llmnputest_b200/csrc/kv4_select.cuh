@@ -11,7 +11,9 @@
 // The bounds are products of a pages x 2 D matrix, the summaries as they lie in memory, with the
 // heads' min(q, 0) and max(q, 0), so the tensor cores take them: mma.sync m16n8k16 of bf16, q in
 // three parts that sum to its 24 bits, 16 pages x 8 heads a warp at a time (16 sequences x 8 kv
-// heads of up to 1024 pages: 14.8 us, and 22.6 with the sums in fp32 FMAs).
+// heads of up to 1024 pages: 14.0 us, where fp32 FMAs took 22.6).  Two CTAs per SM spill 44 and 80 bytes
+// at head_dim 128 and 256; one (162 and 224 registers) makes select and decode of 16 sequences of
+// 1 to 32768 51.3 us instead of 46.5, and 48.9 instead of 44.1.
 //
 // Which page is the n_sel-th may turn on the last bit of two bounds.  With E, a bound on what the
 // fp32 sums are off, the choice is the exact one where the last page taken and the first left out
@@ -22,8 +24,8 @@
 // A cluster per (sequence, kv head): its CTAs take every further group of pages and push the
 // bounds into the first CTA's shared memory, which finds the n_sel-th by 8-bit digits from the
 // highest bit in which they differ, until a digit settles it (two or three rounds), and writes
-// the pages in order.  That tail is what bounds a small call, about 3.5 us of 7.6 for one sequence
-// of 512 pages; the bytes of the summaries would take 2.6 of the 14.8 us.
+// the pages in order.  That tail is what bounds a small call, about 3.5 us of 7.0 for one sequence
+// of 512 pages; the bytes of the summaries would take 2.6 of the 14.0 us.
 #pragma once
 
 #include "kv4_cell.cuh"

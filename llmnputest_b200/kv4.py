@@ -93,7 +93,7 @@ class Kv4Cache:
 
     def positions(self) -> torch.Tensor:
         """Where every row's next token goes: int32 [batch], -1 for a row that is not in use."""
-        return torch.where(self.used > 0, self.lens, -1)
+        return torch.addcmul(self.used - 1, self.lens, self.used)
 
     def compact(self) -> torch.Tensor:
         """Live pages to the lowest numbers (ops.kv4_compact).  Returns info: live pages, pages moved, 0, 0."""
