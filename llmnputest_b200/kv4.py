@@ -47,10 +47,10 @@ class Kv4Cache:
         self.summary = (torch.zeros(n_layers, n_pages, n_kv_heads, 2, head_dim, dtype=torch.bfloat16, device=dev)
                         if summaries else None)
         i32 = dict(dtype=torch.int32, device=dev)
-        self.table = torch.full((batch, max_pages), -1, **i32)
-        self.lens = torch.zeros(batch, **i32)
-        self.refs = torch.zeros(n_pages, **i32)
-        self.info = torch.zeros(4, **i32)
+        # info, counts, lengths and table after one another, as a reorder writes them
+        self._state = torch.zeros(4 + n_pages + batch + batch * max_pages, **i32)
+        self.info, self.refs, self.lens, table = self._state.split((4, n_pages, batch, batch * max_pages))
+        self.table = table.view(batch, max_pages).fill_(-1)
         # 1 for a row in use; one more entry, 0, for those that go on with no row
         self._use = torch.ones(batch + 1, **i32)
         self._use[batch] = 0
@@ -74,12 +74,9 @@ class Kv4Cache:
         return self.info
 
     def _rows(self, parent: torch.Tensor, reserve: torch.Tensor | None) -> None:
-        table, lens, refs, info = ops.kv4_reorder(self.pool, self.table, self.lens, self.refs, parent,
-                                                  head_dim=self.head_dim, reserve=reserve, summary=self.summary)
-        self.table.copy_(table)
-        self.lens.copy_(lens)
-        self.refs.copy_(refs)
-        self.info.copy_(info)
+        anew, at = ops._kv4_reorder(self.pool, self.table, self.lens, self.refs, parent, self.head_dim, reserve,
+                                    self.summary)
+        self._state.copy_(anew[at:])
 
     def reserve(self, tokens: int | torch.Tensor) -> torch.Tensor:
         """Pages for that many tokens behind those that a row has: int32 [batch] (a row with more

@@ -877,6 +877,16 @@ def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, ref
     pool uint8 [layers, n_pages, Hkv, page bytes]; table int32 [B, max_pages]; lens, parent,
     reserve int32 [B]; refs int32 [n_pages].  Returns (table, lens, refs, info) anew; info
     int32 [4]: free pages left, pages copied, pages missing, 0."""
+    anew, at = _kv4_reorder(pool, table, lens, refs, parent, head_dim, reserve, summary, workspace)
+    batch, max_pages = table.shape
+    _, info, refs_out, lens_out, table_out = anew.unsafe_split_with_sizes(
+        (at, 4, refs.numel(), batch, batch * max_pages))
+    return table_out.view(batch, max_pages), lens_out, refs_out, info
+
+
+def _kv4_reorder(pool, table, lens, refs, parent, head_dim, reserve, summary, workspace=None) -> tuple[torch.Tensor, int]:
+    """kv4_reorder's new rows as int32 [4 + n_pages + B + B * max_pages] of one tensor: info, refs,
+    lens and table, from the returned index on."""
     args = _kv4_layers(pool, summary)
     dev, n_pages, page = pool.device, args[-1], _kv4_page(pool.shape[3], head_dim)
     batch, max_pages, pages, length = _kv4_table(table, lens, "lens", dev)
@@ -886,13 +896,14 @@ def kv4_reorder(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, ref
     need = _kv4_ws_bytes(dev.index, "b2_kv4_reorder_workspace_size", batch, max_pages, n_pages)
     # the workspace and the new rows are parts of one allocation
     extra = (need + 15) // 16 * 4 if workspace is None else 0
-    own, info, refs_out, lens_out, table_out = table.new_empty(
-        extra + 4 + n_pages + batch + batch * max_pages).unsafe_split_with_sizes(
-            (extra, 4, n_pages, batch, batch * max_pages))
-    ws, size = (own.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
-    _kv4_call(dev, "b2_kv4_reorder", *args, pages, *rows, batch, max_pages, page, table_out.data_ptr(),
-              lens_out.data_ptr(), refs_out.data_ptr(), info.data_ptr(), ws, size)
-    return table_out.view(batch, max_pages), lens_out, refs_out, info
+    anew = table.new_empty(extra + 4 + n_pages + batch + batch * max_pages)
+    ws, size = (anew.data_ptr(), need) if workspace is None else _kv4_ws_at(workspace, need, dev)
+    info = anew.data_ptr() + 4 * extra
+    refs_out = info + 16
+    lens_out = refs_out + 4 * n_pages
+    _kv4_call(dev, "b2_kv4_reorder", *args, pages, *rows, batch, max_pages, page, lens_out + 4 * batch, lens_out,
+              refs_out, info, ws, size)
+    return anew, extra
 
 
 def kv4_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, *, summary: torch.Tensor | None = None,
