@@ -30,7 +30,7 @@
 // groups of 64 dims.  A group whose own largest weight then lies below 2^-10 is weighed in a unit
 // of its own, a power of two by head and group that its sums carry to the end, so that its w keep
 // fp16's bits too: rare in earnest, so tiles are first taken as if all units were 1 (256 sequences
-// of 2048 of 256 dims 75.5 us so, 73.5 without units, 79.0 with them in every tile).  The sums
+// of 2048 of 256 dims 75.0 us so, 73.5 without units, 79.0 with them in every tile).  The sums
 // L = sum 2^(s - R) and sum 2^(s - R) f stay in fp32; with the least e, 2^-40, the weights 2^(s - R)
 // reach 2^50, and f may be 2^60 in size.
 #pragma once
@@ -318,6 +318,9 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
       st.r[i] = r[i];
     }
     weigh(true);
+    float step[G][2];  // what the groups' units change by
+#pragma unroll
+    for (int g = 0; g < G; ++g) step[g][0] = step[g][1] = 1.f;
     if (G > 1) {  // does every group have a weight near 1, for every head?
       auto most = [&](int g, int i) {
         float x = 0.f;
@@ -354,13 +357,7 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
             float now = x >= kKv4NearOne && x < 2.f ? 1.f : kv4_power_inv(fminf(fmaxf(x, 0x1p-60f), 0x1p60f));
             if (st.r[i] == kKv4NoScore) now = old;  // no score yet
             one = one && now == 1.f;
-            const float f = now * kv4_power_inv(old);
-            st.m[g][i] *= f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              st.o[g][k][i] *= f;
-              st.o[g][k][i + 2] *= f;
-            }
+            step[g][i] = now * kv4_power_inv(old);
             __syncwarp();
             times[g][2 * c + i] = now;  // the same from all lanes of the head
           }
@@ -373,11 +370,12 @@ __device__ __forceinline__ bool kv4_tiles(const uint8_t* tile0, int stride, int 
       st.l[i] *= fall[i];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        st.m[g][i] *= fall[i];
+        const float f = fall[i] * step[g][i];
+        st.m[g][i] *= f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          st.o[g][k][i] *= fall[i];
-          st.o[g][k][i + 2] *= fall[i];
+          st.o[g][k][i] *= f;
+          st.o[g][k][i + 2] *= f;
         }
       }
     }
@@ -441,9 +439,9 @@ __device__ __forceinline__ void kv4_store_out(const Kv4DecodeParams& p, int b, i
 // warps per SM; 55% of the issue slots, 48% of the ALU pipe and 44% of DRAM are used.  64
 // sequences x 8 kv heads of 4096 tokens (152 MB of cache, 23.2 us at the measured HBM rate) take
 // 39.4 us, 3.9 TB/s; 64 x 8 of 2048 of 128 dims (152 MB) 42.5; 256 x 2 of 2048 of 256 dims (305
-// MB, 46.5 us) 75.5 us, 4.0 TB/s.  With a tile's arithmetic left out the rest takes 28.4, 30.1
+// MB, 46.5 us) 75.0 us, 4.1 TB/s.  With a tile's arithmetic left out the rest takes 28.4, 30.1
 // and 57.5; with the copies left out the first takes 37.9.  Measured and dropped, at these three:
-// stages of half the size 45.2, 45.4 and 75.5; three stages (fewer CTAs per SM) 48.7, 56.2 and
+// stages of half the size 45.2, 45.4 and no change; three stages (fewer CTAs per SM) 48.7, 56.2 and
 // 113.8; 5 to 8 CTAs per SM (registers spill); a tile's scores beside the values of the one
 // before.  At D = 64 two tiles are taken at a time (one: 40.4), at 128 one (two: 43.6); at 256
 // one takes 254 registers.  At 128 four CTAs per SM spill 112 bytes, three with 168 registers

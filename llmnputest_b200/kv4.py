@@ -12,7 +12,8 @@
     for l in ...: cache.append(l, k, v, pos); out = cache.decode(l, q, pos, n_q_heads=40)
     cache.advance(1)
     cache.reorder(parent)                            # beams, rows that ended (-1)
-    cache.reorder(same, reserve)                     # a request into a row that ended: its pages
+    cache.reserve(new)                               # a request into a row that ended: its prompt's
+                                                     # length there, 0 for the others
 
 A value takes 4.5 bits (codes of 4 bits, a bf16 step and least value per token, kv head and
 64 dims) where the dense cache of `ops.gqa_decode` takes 16.  Rows share full pages; the table

@@ -160,3 +160,24 @@ def test_nan_with_groups(ops, power):
     assert np.isfinite(got[ok]).all() and ok.sum() == ref.size - 2 * 128 - 2 * 64
     off, size = by_group(np.where(ok, got - ref, 0.0), 64), by_group(np.where(ok, ref, 0.0), 64)
     assert (off <= F32_TOL * size).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_scores_that_jump(ops, dim):
+    """Scores of thousands that rise and fall between pages while the groups' sizes change: only the
+    page of the largest score counts, whatever was summed before it."""
+    rng = np.random.default_rng(dim)
+    c = Case(rng, [16 * 40, 16 * 40], 1, dim, 16, garbage=False)
+    c.cache.meta[..., 0, :, 0] = 2.0 ** -40
+    for b in range(2):
+        for i, at in enumerate(c.table[b, :40]):
+            c.cache.meta[at, ..., 0, :, 1] = [-4.0, 0.5, 2.0, 1.0][i % 4] * (1 + (i == (37 if b else 4)))
+            c.cache.meta[at, :, :, :, 1] *= 2.0 ** rng.choice([0, -25, 20, -35], (1, 1, dim // 64, 1, 1))
+    c.pool = dev(c.cache.pool())
+    q = 1 + np.abs(np.random.default_rng(1).standard_normal((2, 2 * dim))).astype(np.float32)
+    for scale in (100.0, -100.0):
+        ref = c.cache.decode(q.reshape(2, 2, dim), c.table, c.lens - 1, None, scale)
+        got = host(ops.kv4_decode(dev(q), c.pool, c.dtable, c.pos, n_q_heads=2, theta=None, scale=scale, out_f32=True,
+                                  **c.heads))
+        off, size = by_group(got.reshape(ref.shape) - ref, dim), by_group(ref, dim)
+        assert (off <= F32_TOL * size).all(), (scale, (off / size).max())
