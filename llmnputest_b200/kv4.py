@@ -18,11 +18,12 @@
 A value takes 4.5 bits (codes of 4 bits, a bf16 step and least value per token, kv head and
 64 dims) where the dense cache of `ops.gqa_decode` takes 16.  Rows share full pages; the table
 and its counts live on the device and nothing here waits for it: `info` of the last reorder or
-compact can be read when a host wants to know what is free.  A row that a reorder emptied is not
-in use until one reserves pages for it: it takes no page and no token of reserve(1) and
-advance(1), and attends to nothing.  The buffers stay where they are,
-so a captured step sees what later calls put into them.  No reference counterpart (the reference
-keeps one sequence's K and V in bf16, designs/granite_gemv/granite_attention.h:80-213)."""
+compact can be read when a host wants to know what is free.  A row that a reorder emptied, or
+that a new cache's first reserve gave no page, is not in use until pages are reserved for it: it
+takes no page and no token of reserve(1) and advance(1), and attends to nothing.  The buffers
+stay where they are, so a captured step sees what later calls put into them.  No reference
+counterpart (the reference keeps one sequence's K and V in bf16,
+designs/granite_gemv/granite_attention.h:80-213)."""
 
 from __future__ import annotations
 
@@ -52,10 +53,12 @@ class Kv4Cache:
         self._state = torch.zeros(4 + n_pages + batch + batch * max_pages, **i32)
         self.info, self.refs, self.lens, table = self._state.split((4, n_pages, batch, batch * max_pages))
         self.table = table.view(batch, max_pages).fill_(-1)
-        # 1 for a row in use; one more entry, 0, for those that go on with no row
+        # 1 for a row in use; one more entry, 0, for those that go on with no row.  All are until the
+        # first pages are given out: by a tensor, to the rows that begin with them
         self._use = torch.ones(batch + 1, **i32)
         self._use[batch] = 0
         self.used = self._use[:batch]
+        self._fresh = True
         self._same = torch.arange(batch, **i32)
         self._layers = list(self.pool.unbind(0))
         self._near = list(self.summary.unbind(0)) if summaries else [None] * n_layers
@@ -71,8 +74,15 @@ class Kv4Cache:
         self._rows(parent, reserve)
         self.used.copy_(self._use[parent.clamp(-1, self.batch)])  # -1 and batch: the entry that is 0
         if reserve is not None:
-            self.used.logical_or_(reserve > 0)
+            self._begin(reserve)
+        self._fresh = False
         return self.info
+
+    def _begin(self, tokens: torch.Tensor) -> None:
+        if self._fresh and not torch.cuda.is_current_stream_capturing():
+            self.used.copy_(tokens > 0)
+        else:
+            self.used.logical_or_(tokens > 0)
 
     def _rows(self, parent: torch.Tensor, reserve: torch.Tensor | None) -> None:
         anew, at = ops._kv4_reorder(self.pool, self.table, self.lens, self.refs, parent, self.head_dim, reserve,
@@ -81,12 +91,14 @@ class Kv4Cache:
 
     def reserve(self, tokens: int | torch.Tensor) -> torch.Tensor:
         """Pages for that many tokens behind those that a row has: int32 [batch] (a row with more
-        than 0 is in use from then on), or one number for every row in use."""
+        than 0 is in use from then on; where this is a new cache's first call, the others are
+        not), or one number for every row in use (of a new cache: every row)."""
         if isinstance(tokens, torch.Tensor):
             self._rows(self._same, tokens)
-            self.used.logical_or_(tokens > 0)
+            self._begin(tokens)
         else:
             self._rows(self._same, self.used * int(tokens))
+        self._fresh = False
         return self.info
 
     def positions(self) -> torch.Tensor:

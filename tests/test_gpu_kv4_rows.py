@@ -221,3 +221,22 @@ def test_captured_reorders(ops):
         assert s.c.used.tolist() == [int(b in alive) for b in range(3)]
         s.step(alive)
     del g
+
+
+def test_a_row_without_a_first_request(ops):
+    """A batch that begins with a free row: it stays free until a request begins in it.  A cache
+    that begins by one number has all its rows in use."""
+    s = Served()
+    s.prompts([20, 0, 3])
+    for _ in range(17):
+        s.step({0, 2})
+    assert s.pages()[1][1] == 0
+    s.prompts([0, 30, 0])
+    s.step({0, 1, 2})
+    s = Served()
+    s.c.reserve(0)
+    for _ in range(17):
+        s.step({0, 1, 2})
+    s = Served()
+    s.reorder([-1, -1, -1], [4, 0, 0])
+    s.step({0})
